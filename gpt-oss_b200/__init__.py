@@ -39,7 +39,13 @@ EXPORTS = [
     "moe_quantize_mxfp4", "moe_load_layer_f32", "moe_tp_export", "moe_tp_attach_ipc", "moe_tp_buffer", "moe_tp_attach_ptr",
     "moe_tp_forward", "moe_tp_forward_host", "moe_tp_allgather", "moe_tp_reduce_scatter", "moe_tp_allreduce",
     "moe_load_layer_from_bin", "moe_bin_layer_offsets",
+    "moe_route_scored", "moe_group_pairs", "moe_quantize_fp8", "moe_quantize_fp8_blocks", "moe_gemm_fp8", "moe_combine_pairs",
 ]
+
+# Operators of an FP8 expert layer: row types, scores of a routing rule, activations of the quantiser.
+F32, BF16, F16 = range(3)
+SCORE_SOFTMAX, SCORE_SIGMOID = range(2)
+ACT_NONE, ACT_SWIGLU, ACT_SILU_MUL = range(3)
 TP_BUF_GATHER, TP_BUF_PARTIAL, TP_BUF_FLAGS, TP_BUF_TOPK_IDX, TP_BUF_TOPK_W = range(5)
 TP_N_BUFS = 5
 TP_HANDLE_BYTES = 64
@@ -51,6 +57,16 @@ class MoeConfig(C.Structure):
                 ("experts_per_token", C.c_int), ("n_layers", C.c_int), ("swiglu_limit", C.c_float),
                 ("swiglu_alpha", C.c_float), ("max_rows", C.c_int), ("tp_size", C.c_int), ("tp_rank", C.c_int),
                 ("device", C.c_int), ("flags", C.c_uint)]
+
+
+class RouteRule(C.Structure):
+    """moe_route_rule: how moe_route_scored selects experts."""
+    _fields_ = [("n_experts", C.c_int), ("top_k", C.c_int), ("score", C.c_int), ("n_groups", C.c_int),
+                ("top_groups", C.c_int), ("group_top", C.c_int), ("renormalise", C.c_int), ("scale", C.c_float)]
+
+    def __init__(self, n_experts: int, top_k: int, score: int = SCORE_SOFTMAX, n_groups: int = 1, top_groups: int = 1,
+                 group_top: int = 1, renormalise: int = 1, scale: float = 1.0):
+        super().__init__(n_experts, top_k, score, n_groups, top_groups, group_top, renormalise, scale)
 
 
 class MoeError(RuntimeError):
@@ -107,6 +123,14 @@ def lib() -> C.CDLL:
         L.moe_quantize_mxfp4.argtypes = [C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p, C.c_void_p]
         L.moe_load_layer_f32.argtypes = [C.c_void_p, C.c_int] + [C.c_void_p] * 6
         L.moe_block.argtypes = [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_uint, C.c_void_p]
+        ptr, i32, i64 = C.c_void_p, C.c_int, C.c_longlong
+        L.moe_route_scored.argtypes = [ptr, C.POINTER(RouteRule), ptr, i32, i64, ptr, i32, ptr, ptr, ptr]
+        L.moe_group_pairs.argtypes = [ptr, ptr, i32, i32, i32, ptr, ptr, ptr, ptr]
+        L.moe_quantize_fp8.argtypes = [ptr, ptr, i32, i64, i32, i32, i32, C.c_float, C.c_float, ptr, i32, i32, ptr, ptr,
+                                       i64, ptr, i64, ptr]
+        L.moe_quantize_fp8_blocks.argtypes = [ptr, ptr, i32, i64, i32, i32, i32, ptr, i64, ptr, ptr]
+        L.moe_gemm_fp8.argtypes = [ptr, ptr, i64, ptr, i64, i32, ptr, i64, ptr, i32, i32, i32, ptr, ptr, ptr, i32, i64, ptr]
+        L.moe_combine_pairs.argtypes = [ptr, ptr, i32, i64, i32, ptr, ptr, i32, i32, i32, ptr, i64, ptr, i32, i64, ptr]
         L.moe_profile_enable.argtypes = [C.c_void_p, C.c_int]
         L.moe_profile_collect.argtypes = [C.c_void_p, C.POINTER(C.c_float), C.POINTER(C.c_int)]
         _lib = L
@@ -247,6 +271,56 @@ class MoeBlock:
         """Router + top-k + softmax with the library's fixed scratch array; allocates nothing."""
         self._check(self.L.moe_route_static(self.h, layer, C.c_void_p(t_ptr), rows, C.c_void_p(logits_ptr),
                                             C.c_void_p(idx_ptr), C.c_void_p(w_ptr), C.c_void_p(stream)))
+
+    # ---- operators of an FP8 expert layer (device pointers; strides in elements; 0 for an optional pointer) -------
+    def route_scored(self, rule: RouteRule, logits_ptr: int, dtype: int, ld: int, bias_ptr: int, rows: int, idx_ptr: int,
+                     w_ptr: int, stream: int = 0):
+        """Logits [rows, ld] -> experts i32 [rows, top_k] (-1: none left) and weights fp32 [rows, top_k]."""
+        rc = self.L.moe_route_scored(self.h, rule, logits_ptr, dtype, ld, bias_ptr, rows, idx_ptr, w_ptr, stream)
+        if rc:
+            self._check(rc)
+
+    def group_pairs(self, idx_ptr: int, rows: int, top_k: int, n_experts: int, offsets_ptr: int, pair_row_ptr: int,
+                    row_pair_ptr: int = 0, stream: int = 0):
+        """Selections [rows, top_k] -> rows sorted by expert: offsets [n_experts + 1], row of a pair, pair of a row."""
+        rc = self.L.moe_group_pairs(self.h, idx_ptr, rows, top_k, n_experts, offsets_ptr, pair_row_ptr, row_pair_ptr, stream)
+        if rc:
+            self._check(rc)
+
+    def quantize_fp8(self, x_ptr: int, dtype: int, ld_x: int, rows: int, cols: int, codes_ptr: int, ld_codes: int,
+                     scales_ptr: int, ld_scales: int, act: int = ACT_NONE, limit: float = 7.0, alpha: float = 1.702,
+                     pair_row_ptr: int = 0, fanout: int = 1, out_rows: int | None = None, n_rows_ptr: int = 0, stream: int = 0):
+        """Rows (through an activation, to `fanout` places each) -> e4m3 codes and a scale per 128 columns."""
+        rc = self.L.moe_quantize_fp8(self.h, x_ptr, dtype, ld_x, rows, cols, act, limit, alpha, pair_row_ptr, fanout,
+                                     rows if out_rows is None else out_rows, n_rows_ptr, codes_ptr, ld_codes, scales_ptr,
+                                     ld_scales, stream)
+        if rc:
+            self._check(rc)
+
+    def quantize_fp8_blocks(self, w_ptr: int, dtype: int, ld_w: int, n_mats: int, rows: int, cols: int, codes_ptr: int,
+                            ld_codes: int, scales_ptr: int, stream: int = 0):
+        """Weight matrices -> e4m3 codes and a scale per 128 x 128 block."""
+        rc = self.L.moe_quantize_fp8_blocks(self.h, w_ptr, dtype, ld_w, n_mats, rows, cols, codes_ptr, ld_codes, scales_ptr, stream)
+        if rc:
+            self._check(rc)
+
+    def gemm_fp8(self, a_ptr: int, ld_a: int, sa_ptr: int, ld_sa: int, rows: int, b_ptr: int, ld_b: int, sb_ptr: int, n: int,
+                 k: int, out_ptr: int, out_dtype: int, ld_out: int, bias_ptr: int = 0, n_groups: int = 1, offsets_ptr: int = 0,
+                 stream: int = 0):
+        """out [rows, n] = rows x weights^T of their group under both kinds of scales, plus the group's bias."""
+        rc = self.L.moe_gemm_fp8(self.h, a_ptr, ld_a, sa_ptr, ld_sa, rows, b_ptr, ld_b, sb_ptr, n, k, n_groups, offsets_ptr,
+                                 bias_ptr, out_ptr, out_dtype, ld_out, stream)
+        if rc:
+            self._check(rc)
+
+    def combine_pairs(self, y_ptr: int, y_dtype: int, ld_y: int, n_y_rows: int, pair_row_ptr: int, w_ptr: int, rows: int,
+                      top_k: int, cols: int, out_ptr: int, out_dtype: int, ld_out: int, residual_ptr: int = 0,
+                      ld_residual: int = 0, stream: int = 0):
+        """out [rows, cols] = residual + weighted sum of every row's expert rows."""
+        rc = self.L.moe_combine_pairs(self.h, y_ptr, y_dtype, ld_y, n_y_rows, pair_row_ptr, w_ptr, rows, top_k, cols,
+                                      residual_ptr, ld_residual, out_ptr, out_dtype, ld_out, stream)
+        if rc:
+            self._check(rc)
 
     # ---- tensor-parallel group -------------------------------------------------------------
     def tp_export_all(self) -> bytes:

@@ -223,6 +223,80 @@ int moe_tp_allreduce(moe_handle h, void *buf_dev, size_t n_elems, void *stream);
 int moe_route_static(moe_handle h, int layer, const void *t_dev, int rows, float *logits_dev, int *idx_dev,
                      float *w_dev, void *stream);
 
+/* ---- operators of an FP8 expert layer.  No counterpart in the reference, whose experts are MXFP4 and whose router knows one
+ * rule.  A layer whose experts are stored as e4m3 with an fp32 scale per 128 x 128 weights runs, for a batch of rows:
+ *   moe_route_scored -> moe_group_pairs -> moe_quantize_fp8 (pair_row) -> moe_gemm_fp8 -> moe_quantize_fp8 (activation)
+ *   -> moe_gemm_fp8 -> moe_combine_pairs.
+ * All take device pointers on the handle's device and any sizes (the handle's own configuration plays no part), are ordered on
+ * `stream`, allocate nothing, keep nothing between calls, can be captured into a graph, and may overlap one another on the GPU;
+ * zero rows are a valid call that does nothing.  Strides (ld) count elements between rows.  Inputs and outputs of a call must
+ * not overlap, except that moe_combine_pairs may write over its residual (same address, stride and type). */
+enum { MOE_F32 = 0, MOE_BF16 = 1, MOE_F16 = 2 };
+enum { MOE_SCORE_SOFTMAX = 0, MOE_SCORE_SIGMOID = 1 };
+enum { MOE_ACT_NONE = 0, MOE_ACT_SWIGLU = 1, MOE_ACT_SILU_MUL = 2 };
+
+typedef struct moe_route_rule {
+  int n_experts;    /* E <= 512 */
+  int top_k;        /* K <= 32, K <= E */
+  int score;        /* MOE_SCORE_*: s = softmax over the row's experts, or sigmoid */
+  int n_groups;     /* <= 32 equal groups of consecutive experts; 1: no groups */
+  int top_groups;   /* groups that stay */
+  int group_top;    /* 1 or 2: a group is worth the sum of its so many largest s + bias */
+  int renormalise;  /* weights of a row are divided by their sum */
+  float scale;      /* then multiplied by this */
+} moe_route_rule;
+
+/* Routing by scores: logits_dev [rows, ld] of `dtype`, bias_dev fp32 [E] or NULL (it decides the selection, not the weights).
+ * Of the top_groups groups worth most, the K experts with the largest s + bias are selected, largest first, equal ones by the
+ * lower index; comparisons are made in 64 bits.  idx_dev i32 [rows, K], w_dev fp32 [rows, K].  An expert whose logit or bias is
+ * -inf or NaN is off: it is never selected and takes no part in the softmax; +inf counts as the largest finite value.  Where
+ * fewer than K experts are left the rest of the row is index -1 with weight 0. */
+int moe_route_scored(moe_handle h, const moe_route_rule *rule, const void *logits_dev, int dtype, long long ld,
+                     const float *bias_dev, int rows, int *idx_dev, float *w_dev, void *stream);
+
+/* Sorts the pairs p = row * top_k + slot of idx_dev [rows, top_k] by expert (n_experts <= 1024), ascending p inside an expert:
+ * the rows of expert e are [offsets_dev[e], offsets_dev[e + 1]) (i32 [n_experts + 1]), pair p is row pair_row_dev[p], row r is
+ * pair row_pair_dev[r] (i32 [rows * top_k], may be NULL).  A pair whose index is not an expert has row -1; rows from
+ * offsets_dev[n_experts] on are pair -1.  rows * top_k must fit an int. */
+int moe_group_pairs(moe_handle h, const int *idx_dev, int rows, int top_k, int n_experts, int *offsets_dev, int *pair_row_dev,
+                    int *row_pair_dev, void *stream);
+
+/* Rows -> e4m3 codes and fp32 scales, one per 128 columns.  Of a block whose largest finite magnitude is m (at least 2^-96):
+ * scale = m / 448, code = e4m3(v * (448 / m)), rounded to nearest, ties to even.  A NaN has a NaN code, an infinity +-448.
+ * x_dev [rows, ld_x] of `dtype`; act says what v is:
+ *   MOE_ACT_NONE      v[j] = x[j]
+ *   MOE_ACT_SWIGLU    gate = min(x[2j], limit), up = clamp(x[2j+1], -limit, limit): v[j] = gate * sigmoid(alpha * gate) * (up + 1)
+ *   MOE_ACT_SILU_MUL  v[j] = x[j] * sigmoid(x[j]) * x[cols + j]
+ * (`cols` counts v; with an activation x has 2 * cols columns).  Row t is written to the fanout rows pair_row_dev[t, 0..fanout)
+ * of codes_dev [out_rows, ld_codes] and scales_dev [out_rows, ld_scales >= ceil(cols / 128)]; places outside [0, out_rows) are
+ * left out.  Without pair_row_dev row t goes to row t.  n_rows_dev (i32, may be NULL) on the device says how many of the rows
+ * exist; rows, and columns behind `cols`, that nothing is written to keep what they hold. */
+int moe_quantize_fp8(moe_handle h, const void *x_dev, int dtype, long long ld_x, int rows, int cols, int act, float limit,
+                     float alpha, const int *pair_row_dev, int fanout, int out_rows, const int *n_rows_dev, uint8_t *codes_dev,
+                     long long ld_codes, float *scales_dev, long long ld_scales, void *stream);
+
+/* Weights -> e4m3 codes with one scale per 128 x 128 block: n_mats matrices [rows, cols], row strides ld_w and ld_codes, one
+ * behind the other; scales_dev [n_mats, ceil(rows / 128), ceil(cols / 128)].  The same rule as moe_quantize_fp8. */
+int moe_quantize_fp8_blocks(moe_handle h, const void *w_dev, int dtype, long long ld_w, int n_mats, int rows, int cols,
+                            uint8_t *codes_dev, long long ld_codes, float *scales_dev, void *stream);
+
+/* out[m, j] = bias[g, j] + sum over blocks b of 128 of sa[m, b] * sb[g, j / 128, b] * sum over k in b of a[m, k] * w[g, j, k],
+ * products exact, sums in fp32, rounded once to out_dtype.  a_dev e4m3 [rows, ld_a], sa_dev [rows, ld_sa >= ceil(k / 128)],
+ * b_dev e4m3 [n_groups, n, ld_b], sb_dev [n_groups, ceil(n / 128), ceil(k / 128)], bias_dev bf16 [n_groups, n] or NULL.
+ * offsets_dev i32 [n_groups + 1] on the device, ascending: group g (<= 1024) is rows [offsets[g], offsets[g + 1]), output rows
+ * in no group keep what they hold; NULL: one group, all rows.  ld_a and ld_b are multiples of 16 and both code tensors 16-byte
+ * aligned (MOE_ERR_INVALID otherwise); codes behind column k are not looked at. */
+int moe_gemm_fp8(moe_handle h, const uint8_t *a_dev, long long ld_a, const float *sa_dev, long long ld_sa, int rows,
+                 const uint8_t *b_dev, long long ld_b, const float *sb_dev, int n, int k, int n_groups, const int *offsets_dev,
+                 const void *bias_dev, void *out_dev, int out_dtype, long long ld_out, void *stream);
+
+/* out[t] = residual[t] + sum over k of w[t, k] * y[pair_row[t, k]], added in fp32 in the order of k, rounded once.  y_dev
+ * [n_y_rows, ld_y] of y_dtype, pair_row_dev i32 and w_dev fp32 [rows, top_k], residual_dev (may be NULL) and out_dev of out_dtype.
+ * A pair whose row is outside [0, n_y_rows) adds nothing. */
+int moe_combine_pairs(moe_handle h, const void *y_dev, int y_dtype, long long ld_y, int n_y_rows, const int *pair_row_dev,
+                      const float *w_dev, int rows, int top_k, int cols, const void *residual_dev, long long ld_residual,
+                      void *out_dev, int out_dtype, long long ld_out, void *stream);
+
 /* Intermediate results of the last forward, copied to host memory. */
 enum {
   MOE_DBG_LOGITS = 0,   /* f32 [rows, E]    router_score_g */
