@@ -3,88 +3,360 @@
 //
 //   out[m, n] = bias[g, n] + sum over blocks b of  sa[m, b] * sb[g, n / 128, b] * (sum over k in b of a[m, k] * w[g, n, k])
 //
-// with g the group of row m.
+// with g the group of row m.  The inner sum is a tcgen05.mma of K = 128 (four instructions) into a fresh fp32 accumulator in
+// tensor memory; the outer one, with its two scales, is one multiply-add per element and block on the CUDA cores, in fp32
+// registers.
+//
+// The weights are the M operand: a tile is one row of scale blocks (128 weight rows, a lane of tensor memory each) against up
+// to kTok token rows on N, which follows the number of rows of the group in steps of 16.  sb is then one number per tile and
+// block, and sa * sb a vector over the columns of the accumulator that a warp of its own forms in shared memory.
 #include <cuda_fp8.h>
 
 #include "fp8_layer.cuh"
+#include "sm100_ptx.cuh"
 
 namespace moe {
 
+using namespace sm100;
+
 struct Fp8GemmArgs {
-  const uint8_t *a, *b;
-  size_t ld_a, ld_b;         // bytes between rows
   const float *sa, *sb;
   size_t ld_sa;
-  int rows, n, k, n_groups;
+  int rows, n, n_kb, n_groups;
   const int *offsets;        // [n_groups + 1], rows of group g: [offsets[g], offsets[g + 1]); nullptr: one group of all rows
   const __nv_bfloat16 *bias;
   void *out;
   size_t ld_out;
+  int out_dtype;
+  int splits;                // CTAs of a cluster that share the reduction of a tile
+  unsigned int *status;
 };
 
-// Rows [begin, end) of a group, whatever the offsets say inside [0, rows].
-__device__ __forceinline__ void group_rows(const Fp8GemmArgs &p, int g, int &begin, int &end) {
-  begin = 0;
-  end = p.rows;
-  if (p.offsets != nullptr) {
-    begin = min(max(p.offsets[g], 0), p.rows);
-    end = min(max(p.offsets[g + 1], begin), p.rows);
+constexpr int kMaxGemmGroups = 1024;
+constexpr int kGemmRingBytes = 200 * 1024;
+constexpr int kAccBufs = 4;                      // accumulators in tensor memory: blocks of k under way
+constexpr int kScaleSlots = 8;
+constexpr int kWeightTile = kScaleBlock * kScaleBlock;   // bytes of a tile's weights per block of k
+
+template <int kTok>
+struct GemmShape {
+  static constexpr int kBoxRows = kTok <= 32 ? 16 : kTok / 2;     // token rows of a copy
+  static constexpr int kStageBytes = kWeightTile + kTok * kScaleBlock;
+  static constexpr int kStages = kGemmRingBytes / kStageBytes < 12 ? kGemmRingBytes / kStageBytes : 12;
+  static constexpr int kEpiWarps = kTok > 64 ? 8 : 4;
+  static constexpr int kCols = kTok / (kEpiWarps / 4);            // accumulator columns of a warp
+  static constexpr int kBufCols = kTok < 32 ? 32 : kTok;
+  static constexpr int kTmemCols = kAccBufs * kBufCols;
+  static constexpr int kThreads = (kEpiWarps + 3) * 32;           // + copies, MMA, scales
+  static constexpr int kScaleOff = kStages * kStageBytes;
+  static constexpr int kBars = 2 * kStages + 2 * kAccBufs + 2 * kScaleSlots;
+  static constexpr int kBarOff = kScaleOff + kScaleSlots * kTok * 4;
+  static constexpr int kSmem = kBarOff + 8 * kBars + 1024;        // + slack to align the ring
+  static_assert(kTok * kScaleBlock * 4 <= kStages * kStageBytes, "a split's partial tile reuses the ring");
+  static_assert(kSmem + 8 * 1024 <= 227 * 1024, "shared memory");
+};
+
+__device__ __forceinline__ void store_out(const Fp8GemmArgs &p, size_t at, float v) {
+  if (p.out_dtype == MOE_BF16) store_as(static_cast<__nv_bfloat16 *>(p.out) + at, v);
+  else if (p.out_dtype == MOE_F16) store_as(static_cast<__half *>(p.out) + at, v);
+  else store_as(static_cast<float *>(p.out) + at, v);
+}
+
+// One tile: rows [row0, row0 + ntok) of group g against weight rows [128 nb, 128 nb + 128).
+struct GemmTile {
+  int g, nb, row0, ntok;
+};
+
+template <int kTok>
+__global__ void __launch_bounds__(GemmShape<kTok>::kThreads, 1)
+fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const Fp8GemmArgs p) {
+  using S = GemmShape<kTok>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ int s_tiles[kMaxGemmGroups + 1];   // token tiles of the groups before g
+  __shared__ uint32_t s_tmem, s_abort;
+  volatile uint32_t *abort_flag = &s_abort;
+  const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t *ring_ptr = smem_raw + (ring - smem_u32(smem_raw));
+  const uint32_t bars = ring + S::kBarOff;
+  auto full = [&](int s) { return bars + 8u * s; };
+  auto empty = [&](int s) { return bars + 8u * (S::kStages + s); };
+  auto dfull = [&](int d) { return bars + 8u * (2 * S::kStages + d); };
+  auto dempty = [&](int d) { return bars + 8u * (2 * S::kStages + kAccBufs + d); };
+  auto sfull = [&](int s) { return bars + 8u * (2 * S::kStages + 2 * kAccBufs + s); };
+  auto sempty = [&](int s) { return bars + 8u * (2 * S::kStages + 2 * kAccBufs + kScaleSlots + s); };
+  constexpr int kCopyWarp = S::kEpiWarps, kMmaWarp = kCopyWarp + 1, kScaleWarp = kCopyWarp + 2;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::kStages; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
+    for (int d = 0; d < kAccBufs; ++d) { mbar_init(dfull(d), 1); mbar_init(dempty(d), S::kEpiWarps); }
+    for (int s = 0; s < kScaleSlots; ++s) { mbar_init(sfull(s), 1); mbar_init(sempty(s), S::kEpiWarps); }
+    s_abort = 0u;
+    fence_mbar_init();
   }
-}
-
-__device__ __forceinline__ float e4m3_to_f32(uint8_t v) {
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(v), __NV_E4M3)));
-}
-
-// 64 rows x 64 weight rows per CTA on the CUDA cores, a scale block of k at a time through shared memory.
-template <class T>
-__global__ void __launch_bounds__(256)
-fp8_gemm_simt_kernel(const Fp8GemmArgs p) {
-  __shared__ float s_a[32][65], s_b[32][65];
-  int begin, end;
-  group_rows(p, blockIdx.z, begin, end);
-  const int n0 = blockIdx.x * 64, tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  const int n_kb = (p.k + kScaleBlock - 1) / kScaleBlock, n_nb = (p.n + kScaleBlock - 1) / kScaleBlock;
-  for (int m0 = begin + blockIdx.y * 64; m0 < end; m0 += gridDim.y * 64) {
-    float acc[4][4] = {};
-    for (int kb = 0; kb < n_kb; ++kb) {
-      float part[4][4] = {};
-      for (int k0 = kb * kScaleBlock; k0 < min(p.k, (kb + 1) * kScaleBlock); k0 += 32) {
-        __syncthreads();
-        for (int i = threadIdx.x; i < 64 * 32; i += 256) {
-          const int r = i / 32, kk = i % 32;
-          const bool in = k0 + kk < p.k;
-          s_a[kk][r] = in && m0 + r < end ? e4m3_to_f32(p.a[static_cast<size_t>(m0 + r) * p.ld_a + k0 + kk]) : 0.f;
-          s_b[kk][r] = in && n0 + r < p.n ? e4m3_to_f32(p.b[(static_cast<size_t>(blockIdx.z) * p.n + n0 + r) * p.ld_b + k0 + kk]) : 0.f;
-        }
-        __syncthreads();
-        for (int kk = 0; kk < 32; ++kk)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) part[i][j] = fmaf(s_a[kk][ty + 16 * i], s_b[kk][tx + 16 * j], part[i][j]);
+  if (warp == kMmaWarp) {
+    tmem_alloc(smem_u32(&s_tmem), S::kTmemCols);
+    tmem_relinquish();
+  }
+  if (warp == kCopyWarp && lane == 0) {
+    prefetch_tensormap(&tm_a);
+    prefetch_tensormap(&tm_b);
+  }
+  grid_dep_sync();   // from here on what other kernels wrote is read
+  // Token tiles per group, then before every group.  Offsets that are not ascending give wrong rows, never rows outside.
+  auto group_begin = [&](int g) { return p.offsets == nullptr ? 0 : min(max(p.offsets[g], 0), p.rows); };
+  auto group_end = [&](int g) { return p.offsets == nullptr ? p.rows : min(max(p.offsets[g + 1], 0), p.rows); };
+  for (int g = threadIdx.x; g < p.n_groups; g += S::kThreads) s_tiles[g + 1] = (max(group_end(g) - group_begin(g), 0) + kTok - 1) / kTok;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 0) {
+    int before = 0;
+    for (int g0 = 0; g0 < p.n_groups; g0 += 32) {
+      int v = g0 + lane < p.n_groups ? s_tiles[g0 + lane + 1] : 0;
+      for (int off = 1; off < 32; off <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, v, off);
+        if (lane >= off) v += up;
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
-          if (m < end && n < p.n)
-            acc[i][j] = fmaf(part[i][j], p.sa[static_cast<size_t>(m) * p.ld_sa + kb] * p.sb[(static_cast<size_t>(blockIdx.z) * n_nb + n / kScaleBlock) * n_kb + kb], acc[i][j]);
-        }
+      if (g0 + lane < p.n_groups) s_tiles[g0 + lane + 1] = before + v;
+      before += __shfl_sync(0xffffffffu, v, 31);
     }
+    if (lane == 0) s_tiles[0] = 0;
+  }
+  __syncthreads();
+  const uint32_t tmem = s_tmem;
+
+  const int n_nb = (p.n + kScaleBlock - 1) / kScaleBlock;
+  const long long n_items = static_cast<long long>(s_tiles[p.n_groups]) * n_nb;
+  // A split launch has a cluster per tile; otherwise the CTAs walk through the tiles, the token tiles of a weight block next
+  // to one another, so that its weights come from L2 after the first.
+  const int split = p.splits > 1 ? static_cast<int>(blockIdx.y) : 0;
+  const int kb0 = static_cast<int>(static_cast<long long>(p.n_kb) * split / p.splits);
+  const int kb1 = static_cast<int>(static_cast<long long>(p.n_kb) * (split + 1) / p.splits);
+  const long long stride = p.splits > 1 ? n_items + 1 : gridDim.x;   // a split CTA takes one tile
+  auto tile_of = [&](long long item) -> GemmTile {
+    const int q = static_cast<int>(item / n_nb);
+    int lo = 0, hi = p.n_groups;   // s_tiles[lo] <= q < s_tiles[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (s_tiles[mid] <= q) lo = mid; else hi = mid;
+    }
+    const int tiles = s_tiles[lo + 1] - s_tiles[lo];
+    const int local = static_cast<int>(item - static_cast<long long>(s_tiles[lo]) * n_nb);
+    const int begin = group_begin(lo), cnt = group_end(lo) - begin;
+    const int per = ((cnt + tiles - 1) / tiles + 15) / 16 * 16;   // tiles of equal size; at most kTok, none is empty
+    const int row = (local % tiles) * per;
+    return GemmTile{lo, local / tiles, begin + row, min(per, cnt - row)};
+  };
+  bool ok = true;
+
+  if (warp == kCopyWarp) {
+    // ---- copies: the weights of a block of k, and as many boxes of token rows as the tile has
+    uint32_t s = 0, par = 1u;
+    for (long long it = blockIdx.x; ok && it < n_items; it += stride) {
+      const GemmTile t = tile_of(it);
+      const int boxes = (t.ntok + S::kBoxRows - 1) / S::kBoxRows;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait_warp(empty(s), par, abort_flag, p.status, ST_WAIT_EMPTY)) { ok = false; break; }
+        if (elect_one()) {
+          const uint32_t stage = ring + s * S::kStageBytes;
+          mbar_arrive_expect_tx(full(s), kWeightTile + boxes * S::kBoxRows * kScaleBlock);
+          tma_load_3d(stage, &tm_b, kb * kScaleBlock, t.nb * kScaleBlock, t.g, full(s));
+          for (int i = 0; i < boxes; ++i)
+            tma_load_2d(stage + kWeightTile + i * S::kBoxRows * kScaleBlock, &tm_a, kb * kScaleBlock, t.row0 + i * S::kBoxRows, full(s));
+        }
+        __syncwarp();
+        if (++s == S::kStages) { s = 0; par ^= 1u; }
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    // ---- MMA: every block of k into the next of the accumulators
+    uint32_t s = 0, par = 0, d = 0, dpar = 1u;
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const uint64_t desc = smem_desc_sw128(0);
+    for (long long it = blockIdx.x; ok && it < n_items; it += stride) {
+      const GemmTile t = tile_of(it);
+      const uint32_t idesc = idesc_e4m3(kScaleBlock, (t.ntok + 15) / 16 * 16);
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait_warp(dempty(d), dpar, abort_flag, p.status, ST_WAIT_DEMPTY)) { ok = false; break; }
+        if (!mbar_wait_warp(full(s), par, abort_flag, p.status, ST_WAIT_FULL)) { ok = false; break; }
+        tc_fence_after();
+        if (elect_one()) {
+          const uint32_t stage = ring + s * S::kStageBytes, acc = tm + d * S::kBufCols;
+          const uint64_t wd = desc | (stage >> 4), xd = desc | ((stage + kWeightTile) >> 4);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+          for (int i = 0; i < 4; ++i) mma_f8(acc, wd + 2 * i, xd + 2 * i, idesc, i > 0);
+          mma_commit(empty(s));
+          mma_commit(dfull(d));
+        }
+        __syncwarp();
+        if (++s == S::kStages) { s = 0; par ^= 1u; }
+        if (++d == kAccBufs) { d = 0; dpar ^= 1u; }
+      }
+    }
+  } else if (warp == kScaleWarp) {
+    // ---- scales of the tile's tokens times the block's own, one slot per block of k; four blocks are fetched together
+    constexpr int kPer = kTok < 32 ? 1 : kTok / 32, kAhead = 4;
+    uint32_t s = 0, par = 1u;
+    float *slots = reinterpret_cast<float *>(ring_ptr + S::kScaleOff);
+    for (long long it = blockIdx.x; ok && it < n_items; it += stride) {
+      const GemmTile t = tile_of(it);
+      const float *sb = p.sb + (static_cast<size_t>(t.g) * n_nb + t.nb) * p.n_kb;
+      for (int kq = kb0; ok && kq < kb1; kq += kAhead) {
+        float v[kAhead][kPer];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
-        if (m < end && n < p.n) {
-          const float b = p.bias != nullptr ? __bfloat162float(p.bias[static_cast<size_t>(blockIdx.z) * p.n + n]) : 0.f;
-          store_as(static_cast<T *>(p.out) + static_cast<size_t>(m) * p.ld_out + n, acc[i][j] + b);
+        for (int j = 0; j < kAhead; ++j) {
+          const int kb = min(kq + j, kb1 - 1);
+          const float b = sb[kb];
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) {
+            const int tok = lane + 32 * i;
+            v[j][i] = tok < t.ntok ? p.sa[static_cast<size_t>(t.row0 + tok) * p.ld_sa + kb] * b : 0.f;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+          if (!ok || kq + j >= kb1) break;
+          if (!mbar_wait_warp(sempty(s), par, abort_flag, p.status, ST_WAIT_AFREE)) { ok = false; break; }
+#pragma unroll
+          for (int i = 0; i < kPer; ++i)
+            if (lane + 32 * i < kTok) slots[s * kTok + lane + 32 * i] = v[j][i];
+          __syncwarp();
+          if (lane == 0) mbar_arrive(sfull(s));
+          if (++s == kScaleSlots) { s = 0; par ^= 1u; }
         }
       }
+    }
+  } else {
+    // ---- sums over the blocks: warp w holds weight rows 32 (w % 4).. (a lane each) of kCols token columns
+    const int quad = warp & 3, col0 = (warp >> 2) * S::kCols;
+    const uint32_t lane_field = static_cast<uint32_t>(quad * 32) << 16;
+    const float4 *slots = reinterpret_cast<const float4 *>(ring_ptr + S::kScaleOff);
+    uint32_t d = 0, dpar = 0, s = 0, spar = 0;
+    for (long long it = blockIdx.x; ok && it < n_items; it += stride) {
+      const GemmTile t = tile_of(it);
+      const int nrow = t.nb * kScaleBlock + quad * 32 + lane;
+      float acc[S::kCols];
+#pragma unroll
+      for (int c = 0; c < S::kCols; ++c) acc[c] = 0.f;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait_warp(sfull(s), spar, abort_flag, p.status, ST_WAIT_AREADY)) { ok = false; break; }
+        if (!mbar_wait_warp(dfull(d), dpar, abort_flag, p.status, ST_WAIT_DFULL)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t src = tmem + lane_field + d * S::kBufCols + col0;
+        uint32_t v[S::kCols / 16][16];
+#pragma unroll
+        for (int c = 0; c < S::kCols / 16; ++c)
+          if (col0 + 16 * c < t.ntok) tmem_ld16(src + 16 * c, v[c]);
+        tmem_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(dempty(d));
+#pragma unroll
+        for (int c = 0; c < S::kCols / 16; ++c)
+          if (col0 + 16 * c < t.ntok) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float4 f = slots[(s * kTok + col0 + 16 * c) / 4 + i];
+              float *a = acc + 16 * c + 4 * i;
+              a[0] = fmaf(__uint_as_float(v[c][4 * i]), f.x, a[0]);
+              a[1] = fmaf(__uint_as_float(v[c][4 * i + 1]), f.y, a[1]);
+              a[2] = fmaf(__uint_as_float(v[c][4 * i + 2]), f.z, a[2]);
+              a[3] = fmaf(__uint_as_float(v[c][4 * i + 3]), f.w, a[3]);
+            }
+          }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(sempty(s));
+        if (++d == kAccBufs) { d = 0; dpar ^= 1u; }
+        if (++s == kScaleSlots) { s = 0; spar ^= 1u; }
+      }
+      if (!ok) break;
+      if (p.splits > 1) {
+        // every MMA of this CTA is complete: the ring takes the partial tile, [token][weight row]
+        float *part = reinterpret_cast<float *>(ring_ptr);
+#pragma unroll
+        for (int c = 0; c < S::kCols; ++c)
+          if (col0 + c < t.ntok) part[(col0 + c) * kScaleBlock + quad * 32 + lane] = acc[c];
+      } else if (nrow < p.n) {
+        const float b = p.bias != nullptr ? __bfloat162float(p.bias[static_cast<size_t>(t.g) * p.n + nrow]) : 0.f;
+#pragma unroll
+        for (int c = 0; c < S::kCols; ++c)
+          if (col0 + c < t.ntok) store_out(p, static_cast<size_t>(t.row0 + col0 + c) * p.ld_out + nrow, acc[c] + b);
+      }
+    }
+  }
+  __syncwarp();
+  if (p.splits > 1) {
+    // the CTAs of the cluster add up the tile, each its share of the tokens, in the order of k
+    cluster_sync_all();
+    const long long it = blockIdx.x;
+    if (it < n_items) {
+      const GemmTile t = tile_of(it);
+      const uint32_t base = smem_u32(ring_ptr);
+      const int mine = (t.ntok - split + p.splits - 1) / p.splits;
+      for (int e = threadIdx.x; e < mine * kScaleBlock; e += S::kThreads) {
+        const int tok = split + e / kScaleBlock * p.splits, r = e % kScaleBlock, nrow = t.nb * kScaleBlock + r;
+        float sum = 0.f;
+        for (int c = 0; c < p.splits; ++c) sum += ld_cluster_f32(map_to_cta(base + 4u * (tok * kScaleBlock + r), c));
+        if (nrow < p.n) {
+          const float b = p.bias != nullptr ? __bfloat162float(p.bias[static_cast<size_t>(t.g) * p.n + nrow]) : 0.f;
+          store_out(p, static_cast<size_t>(t.row0 + tok) * p.ld_out + nrow, sum + b);
+        }
+      }
+    }
+    cluster_sync_all();   // no CTA leaves while another may still read its part
+  }
+  if (!ok && warp == kCopyWarp)   // give copies in flight time to land before shared memory is released
+    for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, S::kTmemCols);
   }
 }
+
+namespace {
+
+// Codes as rows of k bytes with the 128-byte swizzle of the tensor core: [groups, rows, k], a copy takes box_rows x 128.
+bool encode_codes(CUtensorMap *m, const uint8_t *base, int k, long long ld, int rows, int groups, int box_rows) {
+  TensorMapEncodeFn fn = tensor_map_encoder();
+  if (!fn) return false;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(groups)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld), static_cast<cuuint64_t>(ld) * rows};
+  const cuuint32_t box[3] = {kScaleBlock, static_cast<cuuint32_t>(box_rows), 1}, es[3] = {1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, groups > 0 ? 3 : 2, const_cast<uint8_t *>(base), dims, strides, box, es,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+struct GemmCall {
+  const uint8_t *a, *b;
+  long long ld_a, ld_b;
+  int k;
+  Fp8GemmArgs p;
+};
+
+template <int kTok>
+cudaError_t launch_fp8_gemm(const GemmCall &c, int sm_count, cudaStream_t s, bool &maps_ok) {
+  using S = GemmShape<kTok>;
+  CUtensorMap ma, mb;
+  maps_ok = encode_codes(&ma, c.a, c.k, c.ld_a, c.p.rows, 0, S::kBoxRows) && encode_codes(&mb, c.b, c.k, c.ld_b, c.p.n, c.p.n_groups, kScaleBlock);
+  if (!maps_ok) return cudaSuccess;
+  cudaError_t e = cudaFuncSetAttribute(fp8_gemm_kernel<kTok>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+  if (e != cudaSuccess) return e;
+  // Most tiles that the call can have: a group of cnt rows has at most 1 + (cnt - 1) / kTok.
+  const long long groups = std::min(c.p.n_groups, c.p.rows), n_nb = (c.p.n + kScaleBlock - 1) / kScaleBlock;
+  const long long most = (groups + (c.p.rows - groups) / kTok) * n_nb;
+  Fp8GemmArgs p = c.p;
+  p.splits = 1;
+  while (p.splits < 8 && most * p.splits * 2 <= sm_count && p.splits * 2 <= p.n_kb) p.splits *= 2;
+  const dim3 grid(static_cast<unsigned>(p.splits > 1 ? most : std::min<long long>(most, sm_count)), p.splits, 1);
+  return launch_kernel(fp8_gemm_kernel<kTok>, grid, S::kThreads, S::kSmem, s, true, p.splits > 1 ? p.splits : 0, ma, mb, p);
+}
+
+}  // namespace
 
 }  // namespace moe
 
@@ -109,17 +381,21 @@ int moe_gemm_fp8(moe_handle c, const uint8_t *a_dev, long long ld_a, const float
   if (!aligned_to(sa_dev, 4) || !aligned_to(sb_dev, 4) || !aligned_to(offsets_dev, 4) || !aligned_to(bias_dev, 2) || !aligned_to(out_dev, size))
     return op_fail(c, MOE_ERR_INVALID, "moe_gemm_fp8: a tensor is not aligned to its elements");
   if (int rc = use_device(c, "moe_gemm_fp8")) return rc;
-  Fp8GemmArgs p = {};
-  p.a = a_dev; p.b = b_dev; p.ld_a = static_cast<size_t>(ld_a); p.ld_b = static_cast<size_t>(ld_b);
+  GemmCall call = {a_dev, b_dev, ld_a, ld_b, k, {}};
+  Fp8GemmArgs &p = call.p;
   p.sa = sa_dev; p.sb = sb_dev; p.ld_sa = static_cast<size_t>(ld_sa);
-  p.rows = rows; p.n = n; p.k = k; p.n_groups = n_groups; p.offsets = offsets_dev;
+  p.rows = rows; p.n = n; p.n_kb = static_cast<int>(n_kb); p.n_groups = n_groups; p.offsets = offsets_dev;
   p.bias = static_cast<const __nv_bfloat16 *>(bias_dev); p.out = out_dev; p.ld_out = static_cast<size_t>(ld_out);
-  const dim3 grid((n - 1) / 64 + 1, std::min((rows - 1) / 64 + 1, 128), n_groups);
+  p.out_dtype = out_dtype; p.status = c->status;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (out_dtype == MOE_F32) fp8_gemm_simt_kernel<float><<<grid, 256, 0, s>>>(p);
-  else if (out_dtype == MOE_BF16) fp8_gemm_simt_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(p);
-  else fp8_gemm_simt_kernel<__half><<<grid, 256, 0, s>>>(p);
-  return launched(c, "moe_gemm_fp8", cudaGetLastError());
+  const int per_group = (rows - 1) / n_groups + 1;
+  bool maps_ok = true;
+  const cudaError_t e = per_group <= 16   ? launch_fp8_gemm<16>(call, c->sm_count, s, maps_ok)
+                        : per_group <= 32 ? launch_fp8_gemm<32>(call, c->sm_count, s, maps_ok)
+                        : per_group <= 64 ? launch_fp8_gemm<64>(call, c->sm_count, s, maps_ok)
+                                          : launch_fp8_gemm<128>(call, c->sm_count, s, maps_ok);
+  if (!maps_ok) return op_fail(c, MOE_ERR_INVALID, "moe_gemm_fp8: no tensor map for %d x %d and %d x %d x %d codes", rows, k, n_groups, n, k);
+  return launched(c, "moe_gemm_fp8", e);
 }
 
 }  // extern "C"
