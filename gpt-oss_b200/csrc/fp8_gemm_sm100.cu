@@ -67,6 +67,48 @@ struct GemmTile {
   int g, nb, row0, ntok;
 };
 
+// Offsets that are not ascending give wrong rows, never rows outside.
+__device__ __forceinline__ int group_begin(const Fp8GemmArgs &p, int g) { return p.offsets == nullptr ? 0 : min(max(p.offsets[g], 0), p.rows); }
+__device__ __forceinline__ int group_end(const Fp8GemmArgs &p, int g) { return p.offsets == nullptr ? p.rows : min(max(p.offsets[g + 1], 0), p.rows); }
+
+// s_tiles[g] = token tiles of the groups before g, g = 0..n_groups.  Called by all threads, ends with a barrier.
+template <int kTok>
+__device__ __forceinline__ void count_tiles(const Fp8GemmArgs &p, int *s_tiles) {
+  for (int g = threadIdx.x; g < p.n_groups; g += blockDim.x) s_tiles[g + 1] = (max(group_end(p, g) - group_begin(p, g), 0) + kTok - 1) / kTok;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x;
+    int before = 0;
+    for (int g0 = 0; g0 < p.n_groups; g0 += 32) {
+      int v = g0 + lane < p.n_groups ? s_tiles[g0 + lane + 1] : 0;
+      for (int off = 1; off < 32; off <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, v, off);
+        if (lane >= off) v += up;
+      }
+      if (g0 + lane < p.n_groups) s_tiles[g0 + lane + 1] = before + v;
+      before += __shfl_sync(0xffffffffu, v, 31);
+    }
+    if (lane == 0) s_tiles[0] = 0;
+  }
+  __syncthreads();
+}
+// Item -> tile, of n_nb weight blocks per group: the token tiles of a weight block follow one another.  The tiles of a group
+// are of equal size in steps of 16 rows; none is empty.
+__device__ __forceinline__ GemmTile tile_at(const Fp8GemmArgs &p, const int *s_tiles, long long item, int n_nb) {
+  const int q = static_cast<int>(item / n_nb);
+  int lo = 0, hi = p.n_groups;   // s_tiles[lo] <= q < s_tiles[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (s_tiles[mid] <= q) lo = mid; else hi = mid;
+  }
+  const int tiles = s_tiles[lo + 1] - s_tiles[lo];
+  const int local = static_cast<int>(item - static_cast<long long>(s_tiles[lo]) * n_nb);
+  const int begin = group_begin(p, lo), cnt = group_end(p, lo) - begin;
+  const int per = ((cnt + tiles - 1) / tiles + 15) / 16 * 16;
+  const int row = (local % tiles) * per;
+  return GemmTile{lo, local / tiles, begin + row, min(per, cnt - row)};
+}
+
 template <int kTok>
 __global__ void __launch_bounds__(GemmShape<kTok>::kThreads, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const Fp8GemmArgs p) {
@@ -103,27 +145,9 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
     prefetch_tensormap(&tm_b);
   }
   grid_dep_sync();   // from here on what other kernels wrote is read
-  // Token tiles per group, then before every group.  Offsets that are not ascending give wrong rows, never rows outside.
-  auto group_begin = [&](int g) { return p.offsets == nullptr ? 0 : min(max(p.offsets[g], 0), p.rows); };
-  auto group_end = [&](int g) { return p.offsets == nullptr ? p.rows : min(max(p.offsets[g + 1], 0), p.rows); };
-  for (int g = threadIdx.x; g < p.n_groups; g += S::kThreads) s_tiles[g + 1] = (max(group_end(g) - group_begin(g), 0) + kTok - 1) / kTok;
   tc_fence_before();
-  __syncthreads();
+  count_tiles<kTok>(p, s_tiles);
   tc_fence_after();
-  if (warp == 0) {
-    int before = 0;
-    for (int g0 = 0; g0 < p.n_groups; g0 += 32) {
-      int v = g0 + lane < p.n_groups ? s_tiles[g0 + lane + 1] : 0;
-      for (int off = 1; off < 32; off <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, v, off);
-        if (lane >= off) v += up;
-      }
-      if (g0 + lane < p.n_groups) s_tiles[g0 + lane + 1] = before + v;
-      before += __shfl_sync(0xffffffffu, v, 31);
-    }
-    if (lane == 0) s_tiles[0] = 0;
-  }
-  __syncthreads();
   const uint32_t tmem = s_tmem;
 
   const int n_nb = (p.n + kScaleBlock - 1) / kScaleBlock;
@@ -134,20 +158,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
   const int kb0 = static_cast<int>(static_cast<long long>(p.n_kb) * split / p.splits);
   const int kb1 = static_cast<int>(static_cast<long long>(p.n_kb) * (split + 1) / p.splits);
   const long long stride = p.splits > 1 ? n_items + 1 : gridDim.x;   // a split CTA takes one tile
-  auto tile_of = [&](long long item) -> GemmTile {
-    const int q = static_cast<int>(item / n_nb);
-    int lo = 0, hi = p.n_groups;   // s_tiles[lo] <= q < s_tiles[hi]
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (s_tiles[mid] <= q) lo = mid; else hi = mid;
-    }
-    const int tiles = s_tiles[lo + 1] - s_tiles[lo];
-    const int local = static_cast<int>(item - static_cast<long long>(s_tiles[lo]) * n_nb);
-    const int begin = group_begin(lo), cnt = group_end(lo) - begin;
-    const int per = ((cnt + tiles - 1) / tiles + 15) / 16 * 16;   // tiles of equal size; at most kTok, none is empty
-    const int row = (local % tiles) * per;
-    return GemmTile{lo, local / tiles, begin + row, min(per, cnt - row)};
-  };
+  auto tile_of = [&](long long item) { return tile_at(p, s_tiles, item, n_nb); };
   bool ok = true;
 
   if (warp == kCopyWarp) {
@@ -317,6 +328,229 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
   }
 }
 
+// ---------------------------------------------------------------------------
+// Many rows per group: a pair of CTAs on 256 token rows x 256 weight rows.  Here the token rows are the M operand (a lane of
+// tensor memory each, 128 in either CTA), so that sa * sb is one number per thread and block; each CTA holds half of the
+// weight rows, which the pair's tensor cores share.
+// ---------------------------------------------------------------------------
+constexpr int kPairTok = 256, kPairN = 256;
+constexpr int kPairTile = 128 * kScaleBlock;     // bytes of 128 rows of a block of k: the CTA's token rows, and its weight rows
+constexpr int kPairStage = 2 * kPairTile, kPairStages = 6, kPairAccBufs = 2;
+constexpr int kPairEpiWarps = 8, kPairThreads = (kPairEpiWarps + 4) * 32;
+constexpr int kPairCols = kPairN / (kPairEpiWarps / 4);    // accumulator columns of a warp: one scale block of the weights
+constexpr int kPairBars = 2 * kPairStages + 2 * kPairAccBufs;
+constexpr int kPairSmem = kPairStages * kPairStage + 8 * kPairBars + 1024;
+static_assert(kPairCols == kScaleBlock, "one sb per warp and block of k");
+static_assert(kPairSmem + 8 * 1024 <= 227 * 1024, "shared memory");
+
+__device__ __forceinline__ void fma_f32x2(uint64_t &acc, uint32_t lo, uint32_t hi, uint64_t f) {
+  asm("{\n\t.reg .b64 v;\n\tmov.b64 v, {%1, %2};\n\tfma.rn.f32x2 %0, v, %3, %0;\n\t}" : "+l"(acc) : "r"(lo), "r"(hi), "l"(f));
+}
+
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+// Sixteen consecutive outputs of a row as 32-byte stores.
+template <class T>
+__device__ __forceinline__ void store16(T *dst, const float (&v)[16]) {
+  uint32_t w[16];
+  constexpr int kWords = 4 * static_cast<int>(sizeof(T));
+#pragma unroll
+  for (int i = 0; i < kWords; ++i) {
+    if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(v[i]);
+    else w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+  }
+#pragma unroll
+  for (int i = 0; i < kWords; i += 8)
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(reinterpret_cast<uint32_t *>(dst) + i), "r"(w[i]), "r"(w[i + 1]),
+                 "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7])
+                 : "memory");
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const Fp8GemmArgs p, const int vec_out) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ int s_tiles[kMaxGemmGroups + 1];
+  __shared__ uint32_t s_tmem, s_abort;
+  volatile uint32_t *abort_flag = &s_abort;
+  const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t bars = ring + kPairStages * kPairStage;
+  auto full = [&](int s) { return bars + 8u * s; };
+  auto empty = [&](int s) { return bars + 8u * (kPairStages + s); };
+  auto dfull = [&](int d) { return bars + 8u * (2 * kPairStages + d); };
+  auto dempty = [&](int d) { return bars + 8u * (2 * kPairStages + kPairAccBufs + d); };
+  constexpr int kCopyWarp = kPairEpiWarps, kMmaWarp = kCopyWarp + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(cluster_ctarank());   // 0 issues the MMAs of the pair
+
+  if (threadIdx.x == 0) {
+    // full and dempty are used in the even CTA only: the copies of both CTAs, the epilogue warps of both
+    for (int s = 0; s < kPairStages; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
+    for (int d = 0; d < kPairAccBufs; ++d) { mbar_init(dfull(d), 1); mbar_init(dempty(d), 2 * kPairEpiWarps); }
+    s_abort = 0u;
+    fence_mbar_init();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc_pair(smem_u32(&s_tmem), kPairAccBufs * kPairN);
+    tmem_relinquish_pair();
+  }
+  if (warp == kCopyWarp && lane == 0) {
+    prefetch_tensormap(&tm_a);
+    prefetch_tensormap(&tm_b);
+  }
+  grid_dep_sync();   // from here on what other kernels wrote is read
+  tc_fence_before();
+  count_tiles<kPairTok>(p, s_tiles);
+  cluster_sync_all();   // the peer's barriers exist before anything arrives on them
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  const int n_nb = (p.n + kPairN - 1) / kPairN, n_sb = (p.n + kScaleBlock - 1) / kScaleBlock;
+  const long long n_items = static_cast<long long>(s_tiles[p.n_groups]) * n_nb;
+  const long long first = blockIdx.x >> 1, stride = gridDim.x >> 1;
+  bool ok = true;
+
+  if (warp >= kPairEpiWarps) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == kCopyWarp) {
+      uint32_t s = 0, par = 1u;
+      const uint32_t full0 = map_to_cta(full(0), 0);
+      for (long long it = first; ok && it < n_items; it += stride) {
+        const GemmTile t = tile_at(p, s_tiles, it, n_nb);
+        for (int kb = 0; kb < p.n_kb; ++kb) {
+          if (!mbar_wait_warp<Wait::kClusterRelaxed>(empty(s), par, abort_flag, p.status, ST_WAIT_EMPTY)) { ok = false; break; }
+          if (elect_one()) {
+            const uint32_t stage = ring + s * kPairStage;
+            if (rank == 0) mbar_arrive_expect_tx(full(s), 2 * kPairStage);
+            tma_load_2d_pair(stage, &tm_a, kb * kScaleBlock, t.row0 + 128 * rank, full0 + 8u * s);
+            tma_load_3d_pair(stage + kPairTile, &tm_b, kb * kScaleBlock, t.nb * kPairN + 128 * rank, t.g, full0 + 8u * s);
+          }
+          __syncwarp();
+          if (++s == kPairStages) { s = 0; par ^= 1u; }
+        }
+      }
+    } else if (warp == kMmaWarp && rank == 0) {
+      uint32_t s = 0, par = 0, d = 0, dpar = 1u;
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint64_t desc = smem_desc_sw128(0);
+      constexpr uint32_t idesc = idesc_e4m3(256, kPairN);
+      for (long long it = first; ok && it < n_items; it += stride) {
+        for (int kb = 0; kb < p.n_kb; ++kb) {
+          if (!mbar_wait_warp<Wait::kClusterRelaxed>(dempty(d), dpar, abort_flag, p.status, ST_WAIT_DEMPTY)) { ok = false; break; }
+          if (!mbar_wait_warp<Wait::kCluster>(full(s), par, abort_flag, p.status, ST_WAIT_FULL)) { ok = false; break; }
+          tc_fence_after();
+          if (elect_one()) {
+            const uint32_t stage = ring + s * kPairStage, acc = tm + d * kPairN;
+            const uint64_t xd = desc | (stage >> 4), wd = desc | ((stage + kPairTile) >> 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mma_f8_pair(acc, xd + 2 * i, wd + 2 * i, idesc, i > 0);
+            mma_commit_pair(empty(s));
+            mma_commit_pair(dfull(d));
+          }
+          __syncwarp();
+          if (++s == kPairStages) { s = 0; par ^= 1u; }
+          if (++d == kPairAccBufs) { d = 0; dpar ^= 1u; }
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    const int quad = warp & 3, half = warp >> 2;
+    const uint32_t src0 = tmem + (static_cast<uint32_t>(quad * 32) << 16) + half * kPairCols;
+    const uint32_t dempty0 = map_to_cta(dempty(0), 0);
+    uint32_t d = 0, dpar = 0;
+    for (long long it = first; ok && it < n_items; it += stride) {
+      const GemmTile t = tile_at(p, s_tiles, it, n_nb);
+      const int local = 128 * rank + quad * 32 + lane, n0 = t.nb * kPairN + half * kPairCols;
+      const bool live = local < t.ntok;
+      // a row or weight block that does not exist takes the scales of the last one: its sums go nowhere
+      const float *sa = p.sa + static_cast<size_t>(t.row0 + min(local, t.ntok - 1)) * p.ld_sa;
+      const float *sb = p.sb + (static_cast<size_t>(t.g) * n_sb + min(2 * t.nb + half, n_sb - 1)) * p.n_kb;
+      uint64_t acc[kPairCols / 2];
+#pragma unroll
+      for (int c = 0; c < kPairCols / 2; ++c) acc[c] = 0ull;
+      float f0 = sa[0] * sb[0];
+      float a1 = sa[min(1, p.n_kb - 1)], b1 = sb[min(1, p.n_kb - 1)];
+      for (int kb = 0; kb < p.n_kb; ++kb) {
+        const int ahead = min(kb + 2, p.n_kb - 1);
+        const float a2 = sa[ahead], b2 = sb[ahead];
+        uint64_t f;
+        asm("mov.b64 %0, {%1, %1};" : "=l"(f) : "r"(__float_as_uint(f0)));
+        if (!mbar_wait_warp<Wait::kClusterRelaxed>(dfull(d), dpar, abort_flag, p.status, ST_WAIT_DFULL)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t src = src0 + d * kPairN;
+        uint32_t v[2][32];
+        tmem_ld32(src, v[0]);
+#pragma unroll
+        for (int c = 0; c < kPairCols / 32; ++c) {
+          tmem_wait_ld();
+          if (c + 1 < kPairCols / 32) {
+            tmem_ld32(src + 32 * (c + 1), v[(c + 1) & 1]);
+          } else {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_relaxed_cluster(dempty0 + 8u * d);
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) fma_f32x2(acc[16 * c + i], v[c & 1][2 * i], v[c & 1][2 * i + 1], f);
+        }
+        f0 = a1 * b1;
+        a1 = a2;
+        b1 = b2;
+        if (++d == kPairAccBufs) { d = 0; dpar ^= 1u; }
+      }
+      if (!ok) break;
+      if (live) {
+        const size_t row = static_cast<size_t>(t.row0 + local) * p.ld_out;
+        const __nv_bfloat16 *bias = p.bias != nullptr ? p.bias + static_cast<size_t>(t.g) * p.n : nullptr;
+#pragma unroll
+        for (int c = 0; c < kPairCols / 16; ++c) {
+          const int n = n0 + 16 * c;
+          float o[16];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            o[2 * i] = __uint_as_float(static_cast<uint32_t>(acc[8 * c + i]));
+            o[2 * i + 1] = __uint_as_float(static_cast<uint32_t>(acc[8 * c + i] >> 32));
+          }
+          if (bias != nullptr) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (n + i < p.n) o[i] += __bfloat162float(bias[n + i]);
+          }
+          if (vec_out && n + 16 <= p.n) {
+            if (p.out_dtype == MOE_BF16) store16(static_cast<__nv_bfloat16 *>(p.out) + row + n, o);
+            else if (p.out_dtype == MOE_F16) store16(static_cast<__half *>(p.out) + row + n, o);
+            else store16(static_cast<float *>(p.out) + row + n, o);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (n + i < p.n) store_out(p, row + n + i, o[i]);
+          }
+        }
+      }
+      __syncwarp();
+    }
+  }
+  if (!ok && warp == kCopyWarp)   // give copies in flight time to land before shared memory is released
+    for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();   // neither CTA leaves while the pair's MMAs, copies or arrivals may still touch its memory
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, kPairAccBufs * kPairN);
+  }
+}
+
 namespace {
 
 // Codes as rows of k bytes with the 128-byte swizzle of the tensor core: [groups, rows, k], a copy takes box_rows x 128.
@@ -356,6 +590,20 @@ cudaError_t launch_fp8_gemm(const GemmCall &c, int sm_count, cudaStream_t s, boo
   return launch_kernel(fp8_gemm_kernel<kTok>, grid, S::kThreads, S::kSmem, s, true, p.splits > 1 ? p.splits : 0, ma, mb, p);
 }
 
+cudaError_t launch_fp8_gemm_pair(const GemmCall &c, int sm_count, cudaStream_t s, bool &maps_ok) {
+  CUtensorMap ma, mb;
+  maps_ok = encode_codes(&ma, c.a, c.k, c.ld_a, c.p.rows, 0, 128) && encode_codes(&mb, c.b, c.k, c.ld_b, c.p.n, c.p.n_groups, 128);
+  if (!maps_ok) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(fp8_gemm_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem);
+  if (e != cudaSuccess) return e;
+  const long long groups = std::min(c.p.n_groups, c.p.rows), n_nb = (c.p.n + kPairN - 1) / kPairN;
+  const long long most = (groups + (c.p.rows - groups) / kPairTok) * n_nb;
+  const int size = dtype_size(c.p.out_dtype);
+  const int vec = aligned_to(c.p.out, 32) && c.p.ld_out * size % 32 == 0;
+  return launch_kernel(fp8_gemm_pair_kernel, dim3(2 * static_cast<unsigned>(std::min<long long>(most, sm_count / 2)), 1, 1), kPairThreads, kPairSmem, s,
+                       true, 0, ma, mb, c.p, vec);
+}
+
 }  // namespace
 
 }  // namespace moe
@@ -390,7 +638,8 @@ int moe_gemm_fp8(moe_handle c, const uint8_t *a_dev, long long ld_a, const float
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int per_group = (rows - 1) / n_groups + 1;
   bool maps_ok = true;
-  const cudaError_t e = per_group <= 16   ? launch_fp8_gemm<16>(call, c->sm_count, s, maps_ok)
+  const cudaError_t e = per_group > 96 && n > kScaleBlock ? launch_fp8_gemm_pair(call, c->sm_count, s, maps_ok)
+                        : per_group <= 16   ? launch_fp8_gemm<16>(call, c->sm_count, s, maps_ok)
                         : per_group <= 32 ? launch_fp8_gemm<32>(call, c->sm_count, s, maps_ok)
                         : per_group <= 64 ? launch_fp8_gemm<64>(call, c->sm_count, s, maps_ok)
                                           : launch_fp8_gemm<128>(call, c->sm_count, s, maps_ok);
