@@ -94,15 +94,15 @@ __device__ __forceinline__ void count_tiles(const Fp8GemmArgs &p, int *s_tiles) 
 }
 // Item -> tile, of n_nb weight blocks per group: the token tiles of a weight block follow one another.  The tiles of a group
 // are of equal size in steps of 16 rows; none is empty.
-__device__ __forceinline__ GemmTile tile_at(const Fp8GemmArgs &p, const int *s_tiles, long long item, int n_nb) {
-  const int q = static_cast<int>(item / n_nb);
+__device__ __forceinline__ GemmTile tile_at(const Fp8GemmArgs &p, const int *s_tiles, int item, int n_nb) {
+  const int q = item / n_nb;
   int lo = 0, hi = p.n_groups;   // s_tiles[lo] <= q < s_tiles[hi]
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (s_tiles[mid] <= q) lo = mid; else hi = mid;
   }
   const int tiles = s_tiles[lo + 1] - s_tiles[lo];
-  const int local = static_cast<int>(item - static_cast<long long>(s_tiles[lo]) * n_nb);
+  const int local = item - s_tiles[lo] * n_nb;
   const int begin = group_begin(p, lo), cnt = group_end(p, lo) - begin;
   const int per = ((cnt + tiles - 1) / tiles + 15) / 16 * 16;
   const int row = (local % tiles) * per;
@@ -151,20 +151,20 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
   const uint32_t tmem = s_tmem;
 
   const int n_nb = (p.n + kScaleBlock - 1) / kScaleBlock;
-  const long long n_items = static_cast<long long>(s_tiles[p.n_groups]) * n_nb;
+  const int n_items = s_tiles[p.n_groups] * n_nb;   // far below 2^31: every tile has outputs
   // A split launch has a cluster per tile; otherwise the CTAs walk through the tiles, the token tiles of a weight block next
   // to one another, so that its weights come from L2 after the first.
   const int split = p.splits > 1 ? static_cast<int>(blockIdx.y) : 0;
   const int kb0 = static_cast<int>(static_cast<long long>(p.n_kb) * split / p.splits);
   const int kb1 = static_cast<int>(static_cast<long long>(p.n_kb) * (split + 1) / p.splits);
-  const long long stride = p.splits > 1 ? n_items + 1 : gridDim.x;   // a split CTA takes one tile
-  auto tile_of = [&](long long item) { return tile_at(p, s_tiles, item, n_nb); };
+  const int stride = p.splits > 1 ? n_items : gridDim.x;   // a split CTA takes one tile
+  auto tile_of = [&](int item) { return tile_at(p, s_tiles, item, n_nb); };
   bool ok = true;
 
   if (warp == kCopyWarp) {
     // ---- copies: the weights of a block of k, and as many boxes of token rows as the tile has
     uint32_t s = 0, par = 1u;
-    for (long long it = blockIdx.x; ok && it < n_items; it += stride) {
+    for (int it = blockIdx.x; ok && it < n_items; it += stride) {
       const GemmTile t = tile_of(it);
       const int boxes = (t.ntok + S::kBoxRows - 1) / S::kBoxRows;
       for (int kb = kb0; kb < kb1; ++kb) {
@@ -185,7 +185,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
     uint32_t s = 0, par = 0, d = 0, dpar = 1u;
     const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
     const uint64_t desc = smem_desc_sw128(0);
-    for (long long it = blockIdx.x; ok && it < n_items; it += stride) {
+    for (int it = blockIdx.x; ok && it < n_items; it += stride) {
       const GemmTile t = tile_of(it);
       const uint32_t idesc = idesc_e4m3(kScaleBlock, (t.ntok + 15) / 16 * 16);
       for (int kb = kb0; kb < kb1; ++kb) {
@@ -210,7 +210,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
     constexpr int kPer = kTok < 32 ? 1 : kTok / 32, kAhead = 4;
     uint32_t s = 0, par = 1u;
     float *slots = reinterpret_cast<float *>(ring_ptr + S::kScaleOff);
-    for (long long it = blockIdx.x; ok && it < n_items; it += stride) {
+    for (int it = blockIdx.x; ok && it < n_items; it += stride) {
       const GemmTile t = tile_of(it);
       const float *sb = p.sb + (static_cast<size_t>(t.g) * n_nb + t.nb) * p.n_kb;
       for (int kq = kb0; ok && kq < kb1; kq += kAhead) {
@@ -244,7 +244,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
     const uint32_t lane_field = static_cast<uint32_t>(quad * 32) << 16;
     const float4 *slots = reinterpret_cast<const float4 *>(ring_ptr + S::kScaleOff);
     uint32_t d = 0, dpar = 0, s = 0, spar = 0;
-    for (long long it = blockIdx.x; ok && it < n_items; it += stride) {
+    for (int it = blockIdx.x; ok && it < n_items; it += stride) {
       const GemmTile t = tile_of(it);
       const int nrow = t.nb * kScaleBlock + quad * 32 + lane;
       float acc[S::kCols];
@@ -300,7 +300,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
   if (p.splits > 1) {
     // the CTAs of the cluster add up the tile, each its share of the tokens, in the order of k
     cluster_sync_all();
-    const long long it = blockIdx.x;
+    const int it = blockIdx.x;
     if (it < n_items) {
       const GemmTile t = tile_of(it);
       const uint32_t base = smem_u32(ring_ptr);
@@ -335,11 +335,18 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
 // ---------------------------------------------------------------------------
 constexpr int kPairTok = 256, kPairN = 256;
 constexpr int kPairTile = 128 * kScaleBlock;     // bytes of 128 rows of a block of k: the CTA's token rows, and its weight rows
-constexpr int kPairStage = 2 * kPairTile, kPairStages = 6, kPairAccBufs = 2;
+constexpr int kPairStage = 2 * kPairTile, kPairStages = 4, kPairAccBufs = 2;
 constexpr int kPairEpiWarps = 8, kPairThreads = (kPairEpiWarps + 4) * 32;
 constexpr int kPairCols = kPairN / (kPairEpiWarps / 4);    // accumulator columns of a warp: one scale block of the weights
-constexpr int kPairBars = 2 * kPairStages + 2 * kPairAccBufs;
-constexpr int kPairSmem = kPairStages * kPairStage + 8 * kPairBars + 1024;
+constexpr int kOutBox = 32 * 128, kOutWarp = 2 * kOutBox;  // outputs on their way out: 32 rows of 128 bytes, two a warp
+constexpr int kPairOutOff = kPairStages * kPairStage;
+constexpr int kPairBiasOff = kPairOutOff + kPairEpiWarps * kOutWarp;
+constexpr int kScaleBlocks = 8, kPairScaleSlots = 2;       // blocks of k whose scales are handed over at once
+constexpr int kPairScaleOff = kPairBiasOff + 2 * kPairN * 4;           // [slot][half][block][128 rows]
+constexpr int kPairScaleSlot = 2 * kScaleBlocks * 128;                 // floats
+constexpr int kPairBarOff = kPairScaleOff + kPairScaleSlots * kPairScaleSlot * 4;
+constexpr int kPairBars = 2 * kPairStages + 4 * kPairAccBufs + 2 * kPairScaleSlots + 4;
+constexpr int kPairSmem = kPairBarOff + 8 * kPairBars + 1024;
 static_assert(kPairCols == kScaleBlock, "one sb per warp and block of k");
 static_assert(kPairSmem + 8 * 1024 <= 227 * 1024, "shared memory");
 
@@ -359,43 +366,59 @@ __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t *>(&h);
 }
-// Sixteen consecutive outputs of a row as 32-byte stores.
-template <class T>
-__device__ __forceinline__ void store16(T *dst, const float (&v)[16]) {
-  uint32_t w[16];
-  constexpr int kWords = 4 * static_cast<int>(sizeof(T));
-#pragma unroll
-  for (int i = 0; i < kWords; ++i) {
-    if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(v[i]);
-    else w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+// What the copy engine would do with two boxes of staged outputs (128-byte swizzle), by a warp: rows [0, rows) to output rows
+// row0.. and columns n..; 16 bytes a lane where the output is aligned for it, else an element.
+__device__ __forceinline__ void copy_rows(const Fp8GemmArgs &p, const uint8_t *boxes, int row0, int rows, int n, int box_cols) {
+  const int lane = threadIdx.x & 31, size = p.out_dtype == MOE_F32 ? 4 : 2, per = 16 / size;
+  const bool wide = (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0 && p.ld_out % per == 0;
+  for (int i = lane; i < rows * 16; i += 32) {   // (row, box, 16-byte piece)
+    const int r = i / 16, box = i / 8 % 2, piece = i % 8, col = n + box * box_cols + piece * per;
+    const uint4 v = *reinterpret_cast<const uint4 *>(boxes + box * kOutBox + r * 128 + ((piece ^ (r & 7)) << 4));
+    const size_t at = static_cast<size_t>(row0 + r) * p.ld_out + col;
+    if (wide && col + per <= p.n) {
+      *reinterpret_cast<uint4 *>(static_cast<uint8_t *>(p.out) + at * size) = v;
+    } else {
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      for (int j = 0; j < per; ++j) {
+        if (col + j >= p.n) break;
+        if (size == 4) static_cast<uint32_t *>(p.out)[at + j] = w[j];
+        else static_cast<uint16_t *>(p.out)[at + j] = static_cast<uint16_t>(w[j / 2] >> (16 * (j & 1)));
+      }
+    }
   }
-#pragma unroll
-  for (int i = 0; i < kWords; i += 8)
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(reinterpret_cast<uint32_t *>(dst) + i), "r"(w[i]), "r"(w[i + 1]),
-                 "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7])
-                 : "memory");
 }
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
-fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const Fp8GemmArgs p, const int vec_out) {
+fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_out,
+                     const Fp8GemmArgs p, const int tiled_out) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ int s_tiles[kMaxGemmGroups + 1];
   __shared__ uint32_t s_tmem, s_abort;
   volatile uint32_t *abort_flag = &s_abort;
   const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t bars = ring + kPairStages * kPairStage;
+  float *s_bias = reinterpret_cast<float *>(smem_raw + (ring - smem_u32(smem_raw)) + kPairBiasOff);   // [2][kPairN]
+  float *s_scales = reinterpret_cast<float *>(smem_raw + (ring - smem_u32(smem_raw)) + kPairScaleOff);
+  const uint32_t bars = ring + kPairBarOff;
   auto full = [&](int s) { return bars + 8u * s; };
   auto empty = [&](int s) { return bars + 8u * (kPairStages + s); };
-  auto dfull = [&](int d) { return bars + 8u * (2 * kPairStages + d); };
-  auto dempty = [&](int d) { return bars + 8u * (2 * kPairStages + kPairAccBufs + d); };
-  constexpr int kCopyWarp = kPairEpiWarps, kMmaWarp = kCopyWarp + 1;
+  auto dfull = [&](int h, int d) { return bars + 8u * (2 * kPairStages + kPairAccBufs * h + d); };
+  auto dempty = [&](int h, int d) { return bars + 8u * (2 * kPairStages + kPairAccBufs * (2 + h) + d); };
+  constexpr int kSideBars = 2 * kPairStages + 4 * kPairAccBufs;
+  auto bfull = [&](int i) { return bars + 8u * (kSideBars + i); };
+  auto bempty = [&](int i) { return bars + 8u * (kSideBars + 2 + i); };
+  auto sfull = [&](int i) { return bars + 8u * (kSideBars + 4 + i); };
+  auto sempty = [&](int i) { return bars + 8u * (kSideBars + 4 + kPairScaleSlots + i); };
+  constexpr int kCopyWarp = kPairEpiWarps, kSideWarp = kCopyWarp + 1, kMmaWarp = kCopyWarp + 2;   // two MMA warps
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = static_cast<int>(cluster_ctarank());   // 0 issues the MMAs of the pair
 
   if (threadIdx.x == 0) {
     // full and dempty are used in the even CTA only: the copies of both CTAs, the epilogue warps of both
-    for (int s = 0; s < kPairStages; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
-    for (int d = 0; d < kPairAccBufs; ++d) { mbar_init(dfull(d), 1); mbar_init(dempty(d), 2 * kPairEpiWarps); }
+    for (int s = 0; s < kPairStages; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 2); }
+    for (int h = 0; h < 2; ++h)
+      for (int d = 0; d < kPairAccBufs; ++d) { mbar_init(dfull(h, d), 1); mbar_init(dempty(h, d), kPairEpiWarps); }   // half of either CTA's
+    for (int i = 0; i < 2; ++i) { mbar_init(bfull(i), 1); mbar_init(bempty(i), kPairEpiWarps); }
+    for (int i = 0; i < kPairScaleSlots; ++i) { mbar_init(sfull(i), 1); mbar_init(sempty(i), kPairEpiWarps); }
     s_abort = 0u;
     fence_mbar_init();
   }
@@ -406,6 +429,7 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
   if (warp == kCopyWarp && lane == 0) {
     prefetch_tensormap(&tm_a);
     prefetch_tensormap(&tm_b);
+    if (tiled_out) prefetch_tensormap(&tm_out);
   }
   grid_dep_sync();   // from here on what other kernels wrote is read
   tc_fence_before();
@@ -414,16 +438,15 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
   tc_fence_after();
   const uint32_t tmem = s_tmem;
   const int n_nb = (p.n + kPairN - 1) / kPairN, n_sb = (p.n + kScaleBlock - 1) / kScaleBlock;
-  const long long n_items = static_cast<long long>(s_tiles[p.n_groups]) * n_nb;
-  const long long first = blockIdx.x >> 1, stride = gridDim.x >> 1;
+  const int n_items = s_tiles[p.n_groups] * n_nb;
+  const int first = blockIdx.x >> 1, stride = gridDim.x >> 1;
   bool ok = true;
 
   if (warp >= kPairEpiWarps) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp == kCopyWarp) {
       uint32_t s = 0, par = 1u;
       const uint32_t full0 = map_to_cta(full(0), 0);
-      for (long long it = first; ok && it < n_items; it += stride) {
+      for (int it = first; ok && it < n_items; it += stride) {
         const GemmTile t = tile_at(p, s_tiles, it, n_nb);
         for (int kb = 0; kb < p.n_kb; ++kb) {
           if (!mbar_wait_warp<Wait::kClusterRelaxed>(empty(s), par, abort_flag, p.status, ST_WAIT_EMPTY)) { ok = false; break; }
@@ -431,29 +454,32 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
             const uint32_t stage = ring + s * kPairStage;
             if (rank == 0) mbar_arrive_expect_tx(full(s), 2 * kPairStage);
             tma_load_2d_pair(stage, &tm_a, kb * kScaleBlock, t.row0 + 128 * rank, full0 + 8u * s);
-            tma_load_3d_pair(stage + kPairTile, &tm_b, kb * kScaleBlock, t.nb * kPairN + 128 * rank, t.g, full0 + 8u * s);
+            for (int h = 0; h < 2; ++h)   // 64 of the 128 weight rows of either half
+              tma_load_3d_pair(stage + kPairTile + h * (kPairTile / 2), &tm_b, kb * kScaleBlock, t.nb * kPairN + 128 * h + 64 * rank, t.g, full0 + 8u * s);
           }
           __syncwarp();
           if (++s == kPairStages) { s = 0; par ^= 1u; }
         }
       }
-    } else if (warp == kMmaWarp && rank == 0) {
+    } else if (warp >= kMmaWarp && rank == 0) {
+      // ---- MMA: a warp for either half of the columns, with accumulators of its own
+      const int half = warp - kMmaWarp;
       uint32_t s = 0, par = 0, d = 0, dpar = 1u;
-      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0) + half * kPairAccBufs * kPairCols;
       const uint64_t desc = smem_desc_sw128(0);
-      constexpr uint32_t idesc = idesc_e4m3(256, kPairN);
-      for (long long it = first; ok && it < n_items; it += stride) {
+      constexpr uint32_t idesc = idesc_e4m3(256, kPairCols);
+      for (int it = first; ok && it < n_items; it += stride) {
         for (int kb = 0; kb < p.n_kb; ++kb) {
-          if (!mbar_wait_warp<Wait::kClusterRelaxed>(dempty(d), dpar, abort_flag, p.status, ST_WAIT_DEMPTY)) { ok = false; break; }
           if (!mbar_wait_warp<Wait::kCluster>(full(s), par, abort_flag, p.status, ST_WAIT_FULL)) { ok = false; break; }
+          if (!mbar_wait_warp<Wait::kClusterRelaxed>(dempty(half, d), dpar, abort_flag, p.status, ST_WAIT_DEMPTY)) { ok = false; break; }
           tc_fence_after();
           if (elect_one()) {
-            const uint32_t stage = ring + s * kPairStage, acc = tm + d * kPairN;
-            const uint64_t xd = desc | (stage >> 4), wd = desc | ((stage + kPairTile) >> 4);
+            const uint32_t stage = ring + s * kPairStage, acc = tm + d * kPairCols;
+            const uint64_t xd = desc | (stage >> 4), wd = desc | ((stage + kPairTile + half * (kPairTile / 2)) >> 4);
 #pragma unroll
             for (int i = 0; i < 4; ++i) mma_f8_pair(acc, xd + 2 * i, wd + 2 * i, idesc, i > 0);
+            mma_commit_pair(dfull(half, d));
             mma_commit_pair(empty(s));
-            mma_commit_pair(dfull(d));
           }
           __syncwarp();
           if (++s == kPairStages) { s = 0; par ^= 1u; }
@@ -461,83 +487,157 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
         }
       }
     }
+    if (warp == kSideWarp) {
+      // ---- bias as fp32, and the products of both scales: for every row of this CTA and either half of the columns
+      uint32_t buf = 0, bpar = 1u, s = 0, par = 1u;
+      for (int it = first; ok && it < n_items; it += stride) {
+        const GemmTile t = tile_at(p, s_tiles, it, n_nb);
+        // rows and weight blocks that do not exist take the scales of the last one: their sums go nowhere
+        const float *sb0 = p.sb + (static_cast<size_t>(t.g) * n_sb + 2 * t.nb) * p.n_kb, *sb1 = 2 * t.nb + 1 < n_sb ? sb0 + p.n_kb : sb0;
+        float bias[kPairN / 32];
+#pragma unroll
+        for (int i = 0; i < kPairN / 32; ++i) {
+          const int n = t.nb * kPairN + 32 * i + lane;
+          bias[i] = p.bias != nullptr && n < p.n ? __bfloat162float(p.bias[static_cast<size_t>(t.g) * p.n + n]) : 0.f;
+        }
+        for (int k0 = 0; ok && k0 < p.n_kb; k0 += kScaleBlocks) {
+          const bool mine = lane < kScaleBlocks && k0 + lane < p.n_kb;
+          const float b0 = mine ? sb0[k0 + lane] : 0.f, b1 = mine ? sb1[k0 + lane] : 0.f;
+          float v[4][kScaleBlocks];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float *sa = p.sa + static_cast<size_t>(t.row0 + min(128 * rank + 32 * r + lane, t.ntok - 1)) * p.ld_sa + k0;
+#pragma unroll
+            for (int j = 0; j < kScaleBlocks; ++j) v[r][j] = k0 + j < p.n_kb ? sa[j] : 0.f;
+          }
+          if (!mbar_wait_warp(sempty(s), par, abort_flag, p.status, ST_WAIT_AFREE)) { ok = false; break; }
+          float *dst = s_scales + s * kPairScaleSlot + lane;
+#pragma unroll
+          for (int j = 0; j < kScaleBlocks; ++j) {
+            const float f0 = __shfl_sync(0xffffffffu, b0, j), f1 = __shfl_sync(0xffffffffu, b1, j);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              dst[j * 128 + 32 * r] = v[r][j] * f0;
+              dst[(kScaleBlocks + j) * 128 + 32 * r] = v[r][j] * f1;
+            }
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(sfull(s));
+          if (++s == kPairScaleSlots) { s = 0; par ^= 1u; }
+        }
+        if (!ok || !mbar_wait_warp(bempty(buf), bpar, abort_flag, p.status, ST_WAIT_AFREE)) { ok = false; break; }
+#pragma unroll
+        for (int i = 0; i < kPairN / 32; ++i) s_bias[buf * kPairN + 32 * i + lane] = bias[i];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bfull(buf));
+        if (buf ^= 1u; buf == 0) bpar ^= 1u;
+      }
+    }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     const int quad = warp & 3, half = warp >> 2;
-    const uint32_t src0 = tmem + (static_cast<uint32_t>(quad * 32) << 16) + half * kPairCols;
-    const uint32_t dempty0 = map_to_cta(dempty(0), 0);
-    uint32_t d = 0, dpar = 0;
-    for (long long it = first; ok && it < n_items; it += stride) {
+    const uint32_t src0 = tmem + (static_cast<uint32_t>(quad * 32) << 16) + half * kPairAccBufs * kPairCols;
+    const uint32_t dempty0 = map_to_cta(dempty(half, 0), 0);
+    const uint32_t out_smem = ring + kPairOutOff + warp * kOutWarp;
+    const uint32_t out_lane = out_smem + lane * 128 + ((lane & 7) << 4);   // piece i of the lane's row: at this address ^ 16 i
+    const uint8_t *out_gen = smem_raw + (out_smem - smem_u32(smem_raw));
+    uint32_t d = 0, dpar = 0, buf = 0, bpar = 0, s = 0, spar = 0;
+    for (int it = first; it < n_items; it += stride) {
       const GemmTile t = tile_at(p, s_tiles, it, n_nb);
-      const int local = 128 * rank + quad * 32 + lane, n0 = t.nb * kPairN + half * kPairCols;
-      const bool live = local < t.ntok;
-      // a row or weight block that does not exist takes the scales of the last one: its sums go nowhere
-      const float *sa = p.sa + static_cast<size_t>(t.row0 + min(local, t.ntok - 1)) * p.ld_sa;
-      const float *sb = p.sb + (static_cast<size_t>(t.g) * n_sb + min(2 * t.nb + half, n_sb - 1)) * p.n_kb;
+      const int n0 = t.nb * kPairN + half * kPairCols;
       uint64_t acc[kPairCols / 2];
 #pragma unroll
       for (int c = 0; c < kPairCols / 2; ++c) acc[c] = 0ull;
-      float f0 = sa[0] * sb[0];
-      float a1 = sa[min(1, p.n_kb - 1)], b1 = sb[min(1, p.n_kb - 1)];
       for (int kb = 0; kb < p.n_kb; ++kb) {
-        const int ahead = min(kb + 2, p.n_kb - 1);
-        const float a2 = sa[ahead], b2 = sb[ahead];
+        if (kb % kScaleBlocks == 0 && !mbar_wait_warp(sfull(s), spar, abort_flag, p.status, ST_WAIT_AREADY)) { ok = false; break; }
+        const float scale = s_scales[s * kPairScaleSlot + (half * kScaleBlocks + kb % kScaleBlocks) * 128 + quad * 32 + lane];
         uint64_t f;
-        asm("mov.b64 %0, {%1, %1};" : "=l"(f) : "r"(__float_as_uint(f0)));
-        if (!mbar_wait_warp<Wait::kClusterRelaxed>(dfull(d), dpar, abort_flag, p.status, ST_WAIT_DFULL)) { ok = false; break; }
+        asm("mov.b64 %0, {%1, %1};" : "=l"(f) : "r"(__float_as_uint(scale)));
+        if (!mbar_wait_warp<Wait::kClusterRelaxed>(dfull(half, d), dpar, abort_flag, p.status, ST_WAIT_DFULL)) { ok = false; break; }
         tc_fence_after();
-        const uint32_t src = src0 + d * kPairN;
-        uint32_t v[2][32];
-        tmem_ld32(src, v[0]);
+        const uint32_t src = src0 + d * kPairCols;
+        uint32_t v[2][16];
+        tmem_ld16(src, v[0]);
 #pragma unroll
-        for (int c = 0; c < kPairCols / 32; ++c) {
+        for (int c = 0; c < kPairCols / 16; ++c) {   // the next 16 columns are on their way while these are added
           tmem_wait_ld();
-          if (c + 1 < kPairCols / 32) {
-            tmem_ld32(src + 32 * (c + 1), v[(c + 1) & 1]);
+          if (c + 1 < kPairCols / 16) {
+            tmem_ld16(src + 16 * (c + 1), v[(c + 1) & 1]);
           } else {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_relaxed_cluster(dempty0 + 8u * d);
           }
 #pragma unroll
-          for (int i = 0; i < 16; ++i) fma_f32x2(acc[16 * c + i], v[c & 1][2 * i], v[c & 1][2 * i + 1], f);
+          for (int i = 0; i < 8; ++i) fma_f32x2(acc[8 * c + i], v[c & 1][2 * i], v[c & 1][2 * i + 1], f);
         }
-        f0 = a1 * b1;
-        a1 = a2;
-        b1 = b2;
+        if (kb % kScaleBlocks == kScaleBlocks - 1 || kb + 1 == p.n_kb) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(sempty(s));
+          if (++s == kPairScaleSlots) { s = 0; spar ^= 1u; }
+        }
         if (++d == kPairAccBufs) { d = 0; dpar ^= 1u; }
       }
       if (!ok) break;
-      if (live) {
-        const size_t row = static_cast<size_t>(t.row0 + local) * p.ld_out;
-        const __nv_bfloat16 *bias = p.bias != nullptr ? p.bias + static_cast<size_t>(t.g) * p.n : nullptr;
-#pragma unroll
-        for (int c = 0; c < kPairCols / 16; ++c) {
-          const int n = n0 + 16 * c;
-          float o[16];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            o[2 * i] = __uint_as_float(static_cast<uint32_t>(acc[8 * c + i]));
-            o[2 * i + 1] = __uint_as_float(static_cast<uint32_t>(acc[8 * c + i] >> 32));
+      // Through shared memory, boxes of 32 rows x 128 bytes: two of 64 16-bit columns, or twice two of 32 fp32 columns.  Rows
+      // that all exist leave by the copy engine while the next tile is under way, others (and outputs that it cannot
+      // address) by the warp, a row at a time.
+      const int rows_here = t.ntok - 128 * rank - quad * 32, row_out = t.row0 + 128 * rank + quad * 32;
+      const bool by_copy = tiled_out && rows_here >= 32;
+      auto leave = [&](int n, int box_cols) {   // both boxes, columns n..
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (by_copy) {
+          if (lane == 0) {
+            for (int i = 0; i < 2; ++i)
+              if (n + i * box_cols < p.n) tma_store_2d(&tm_out, n + i * box_cols, row_out, out_smem + i * kOutBox);
+            tma_store_commit();
           }
-          if (bias != nullptr) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (n + i < p.n) o[i] += __bfloat162float(bias[n + i]);
-          }
-          if (vec_out && n + 16 <= p.n) {
-            if (p.out_dtype == MOE_BF16) store16(static_cast<__nv_bfloat16 *>(p.out) + row + n, o);
-            else if (p.out_dtype == MOE_F16) store16(static_cast<__half *>(p.out) + row + n, o);
-            else store16(static_cast<float *>(p.out) + row + n, o);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (n + i < p.n) store_out(p, row + n + i, o[i]);
-          }
+        } else {
+          copy_rows(p, out_gen, row_out, min(rows_here, 32), n, box_cols);
         }
+      };
+      // (the address is formed inside the statement: sixteen of them, kept across the loop over k, would cost registers there)
+      auto stage = [&](int box, int piece, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
+        asm volatile("{\n\t.reg .b32 at;\n\txor.b32 at, %0, %1;\n\tadd.u32 at, at, %2;\n\tst.shared.v4.b32 [at], {%3, %4, %5, %6};\n\t}" ::"r"(out_lane),
+                     "r"(piece << 4), "r"(box * kOutBox), "r"(w0), "r"(w1), "r"(w2), "r"(w3)
+                     : "memory");
+      };
+      if (!mbar_wait_warp(bfull(buf), bpar, abort_flag, p.status, ST_WAIT_AREADY)) { ok = false; break; }
+      const float4 *bias = reinterpret_cast<const float4 *>(s_bias + buf * kPairN + half * kPairCols);
+      auto sums = [&](int c) {   // four columns with their bias
+        const float4 b = bias[c];
+        return make_float4(__uint_as_float(static_cast<uint32_t>(acc[2 * c])) + b.x, __uint_as_float(static_cast<uint32_t>(acc[2 * c] >> 32)) + b.y,
+                           __uint_as_float(static_cast<uint32_t>(acc[2 * c + 1])) + b.z, __uint_as_float(static_cast<uint32_t>(acc[2 * c + 1] >> 32)) + b.w);
+      };
+      if (lane == 0) tma_store_wait_read();   // of the tile before
+      __syncwarp();
+      if (p.out_dtype == MOE_F32) {
+#pragma unroll
+        for (int c = 0; c < kPairCols / 4; ++c) {
+          if (c == kPairCols / 8) {
+            leave(n0, 32);
+            if (lane == 0) tma_store_wait_read();
+            __syncwarp();
+          }
+          const float4 v = sums(c);
+          stage(c / 8 % 2, c % 8, __float_as_uint(v.x), __float_as_uint(v.y), __float_as_uint(v.z), __float_as_uint(v.w));
+        }
+        leave(n0 + kPairCols / 2, 32);
+      } else {
+        const bool bf16 = p.out_dtype == MOE_BF16;
+        auto pack = [&](float lo, float hi) { return bf16 ? pack2<__nv_bfloat16>(lo, hi) : pack2<__half>(lo, hi); };
+#pragma unroll
+        for (int c = 0; c < kPairCols / 8; ++c) {
+          const float4 v = sums(2 * c), u = sums(2 * c + 1);
+          stage(c / 8, c % 8, pack(v.x, v.y), pack(v.z, v.w), pack(u.x, u.y), pack(u.z, u.w));
+        }
+        leave(n0, 64);
       }
       __syncwarp();
+      if (lane == 0) mbar_arrive(bempty(buf));
+      if (buf ^= 1u; buf == 0) bpar ^= 1u;
     }
+    if (lane == 0) tma_store_wait_all();
   }
   if (!ok && warp == kCopyWarp)   // give copies in flight time to land before shared memory is released
     for (int i = 0; i < 2000; ++i) __nanosleep(1000);
@@ -563,6 +663,17 @@ bool encode_codes(CUtensorMap *m, const uint8_t *base, int k, long long ld, int 
   return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, groups > 0 ? 3 : 2, const_cast<uint8_t *>(base), dims, strides, box, es,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Outputs [rows, n], stored as boxes of 32 rows x 128 bytes.
+bool encode_out(CUtensorMap *m, const Fp8GemmArgs &p) {
+  TensorMapEncodeFn fn = tensor_map_encoder();
+  if (!fn) return false;
+  const int size = dtype_size(p.out_dtype);
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(p.n), static_cast<cuuint64_t>(p.rows)}, strides[1] = {static_cast<cuuint64_t>(p.ld_out) * size};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / size), 32}, es[2] = {1, 1};
+  return fn(m, size == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, p.out, dims, strides, box, es,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 struct GemmCall {
@@ -592,16 +703,17 @@ cudaError_t launch_fp8_gemm(const GemmCall &c, int sm_count, cudaStream_t s, boo
 
 cudaError_t launch_fp8_gemm_pair(const GemmCall &c, int sm_count, cudaStream_t s, bool &maps_ok) {
   CUtensorMap ma, mb;
-  maps_ok = encode_codes(&ma, c.a, c.k, c.ld_a, c.p.rows, 0, 128) && encode_codes(&mb, c.b, c.k, c.ld_b, c.p.n, c.p.n_groups, 128);
+  maps_ok = encode_codes(&ma, c.a, c.k, c.ld_a, c.p.rows, 0, 128) && encode_codes(&mb, c.b, c.k, c.ld_b, c.p.n, c.p.n_groups, 64);
   if (!maps_ok) return cudaSuccess;
   const cudaError_t e = cudaFuncSetAttribute(fp8_gemm_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem);
   if (e != cudaSuccess) return e;
   const long long groups = std::min(c.p.n_groups, c.p.rows), n_nb = (c.p.n + kPairN - 1) / kPairN;
   const long long most = (groups + (c.p.rows - groups) / kPairTok) * n_nb;
-  const int size = dtype_size(c.p.out_dtype);
-  const int vec = aligned_to(c.p.out, 32) && c.p.ld_out * size % 32 == 0;
+  // outputs through the copy engine: rows of 16-byte pieces
+  CUtensorMap mo = ma;
+  const int tiled = aligned_to(c.p.out, 16) && c.p.ld_out * dtype_size(c.p.out_dtype) % 16 == 0 && encode_out(&mo, c.p);
   return launch_kernel(fp8_gemm_pair_kernel, dim3(2 * static_cast<unsigned>(std::min<long long>(most, sm_count / 2)), 1, 1), kPairThreads, kPairSmem, s,
-                       true, 0, ma, mb, c.p, vec);
+                       true, 0, ma, mb, mo, c.p, tiled);
 }
 
 }  // namespace
