@@ -9,7 +9,9 @@
 //
 // The weights are the M operand: a tile is one row of scale blocks (128 weight rows, a lane of tensor memory each) against up
 // to kTok token rows on N, which follows the number of rows of the group in steps of 16.  sb is then one number per tile and
-// block, and sa * sb a vector over the columns of the accumulator that a warp of its own forms in shared memory.
+// block, and sa * sb a vector over the columns of the accumulator that a warp of its own forms in shared memory.  The
+// accumulators are read as fragments (a thread has two neighbouring columns of four rows): an 8-byte load of scales then serves
+// four packed multiply-adds, where a row per thread would load every scale of the tile in every thread.
 #include <cuda_fp8.h>
 
 #include "fp8_layer.cuh"
@@ -33,33 +35,73 @@ struct Fp8GemmArgs {
 };
 
 constexpr int kMaxGemmGroups = 1024;
-constexpr int kGemmRingBytes = 200 * 1024;
-constexpr int kAccBufs = 4;                      // accumulators in tensor memory: blocks of k under way
-constexpr int kScaleSlots = 8;
+constexpr int kGemmRingBytes = 218 * 1024;               // of shared memory for tiles, scales and outputs
+constexpr int kScaleBlocks = 8, kScaleSlots = 2;         // blocks of k whose scales are handed over at once
 constexpr int kWeightTile = kScaleBlock * kScaleBlock;   // bytes of a tile's weights per block of k
 
 template <int kTok>
 struct GemmShape {
   static constexpr int kBoxRows = kTok <= 32 ? 16 : kTok / 2;     // token rows of a copy
   static constexpr int kStageBytes = kWeightTile + kTok * kScaleBlock;
-  static constexpr int kStages = kGemmRingBytes / kStageBytes < 12 ? kGemmRingBytes / kStageBytes : 12;
-  static constexpr int kEpiWarps = kTok > 64 ? 8 : 4;
+  static constexpr int kEpiWarps = kTok <= 64 ? 4 : kTok / 16;
   static constexpr int kCols = kTok / (kEpiWarps / 4);            // accumulator columns of a warp
+  static constexpr int kChunk = kCols < 32 ? kCols : kTok > 128 ? 32 : kCols;   // of these, fetched from tensor memory at once
   static constexpr int kBufCols = kTok < 32 ? 32 : kTok;
-  static constexpr int kTmemCols = kAccBufs * kBufCols;
+  static constexpr int kAccBufs = kTok > 128 ? 2 : 4;             // accumulators: blocks of k under way
+  static constexpr int kTmemCols = kTok > 128 ? 512 : kAccBufs * kBufCols;   // a power of two
   static constexpr int kThreads = (kEpiWarps + 3) * 32;           // + copies, MMA, scales
+  static constexpr int kPartPitch = kScaleBlock + 4;              // floats of a token's partial sums: no bank conflicts
+  static constexpr int kOutPitch = 80;                            // bytes of 32 16-bit outputs of a token, the same
+  static constexpr int kOutCols = kCols < 32 ? kCols : 32;        // tokens of a warp that are on their way out at once
+  static constexpr int kOutWarp = kOutCols * kOutPitch;
+  static constexpr int kRing = kGemmRingBytes - kEpiWarps * kOutWarp - kScaleSlots * kScaleBlocks * kTok * 4;
+  static constexpr int kStages = kRing / kStageBytes < 12 ? kRing / kStageBytes : 12;
   static constexpr int kScaleOff = kStages * kStageBytes;
-  static constexpr int kBars = 2 * kStages + 2 * kAccBufs + 2 * kScaleSlots;
-  static constexpr int kBarOff = kScaleOff + kScaleSlots * kTok * 4;
+  static constexpr int kOutOff = kScaleOff + kScaleSlots * kScaleBlocks * kTok * 4;
+  static constexpr int kPlanOff = kOutOff + kEpiWarps * kOutWarp;  // [2]: a tile's GemmTile and the bias of its weight rows
+  static constexpr int kPlanBytes = 16 + kScaleBlock * 4;
+  static constexpr int kBarOff = kPlanOff + 2 * kPlanBytes;
+  static constexpr int kBars = 2 * kStages + 2 * kAccBufs + 2 * kScaleSlots + 4;
   static constexpr int kSmem = kBarOff + 8 * kBars + 1024;        // + slack to align the ring
-  static_assert(kTok * kScaleBlock * 4 <= kStages * kStageBytes, "a split's partial tile reuses the ring");
-  static_assert(kSmem + 8 * 1024 <= 227 * 1024, "shared memory");
+  static_assert(kTok * kPartPitch * 4 <= kStages * kStageBytes, "a split's partial tile reuses the ring");
+  static_assert(kSmem + 4608 <= 227 * 1024, "shared memory");
 };
 
+__device__ __forceinline__ void fma_f32x2(uint64_t &acc, uint32_t lo, uint32_t hi, uint64_t f) {
+  asm("{\n\t.reg .b64 v;\n\tmov.b64 v, {%1, %2};\n\tfma.rn.f32x2 %0, v, %3, %0;\n\t}" : "+l"(acc) : "r"(lo), "r"(hi), "l"(f));
+}
+
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
 __device__ __forceinline__ void store_out(const Fp8GemmArgs &p, size_t at, float v) {
   if (p.out_dtype == MOE_BF16) store_as(static_cast<__nv_bfloat16 *>(p.out) + at, v);
   else if (p.out_dtype == MOE_F16) store_as(static_cast<__half *>(p.out) + at, v);
   else store_as(static_cast<float *>(p.out) + at, v);
+}
+
+// Four neighbouring sums of a tile whose reduction is split: the parts of all CTAs of the cluster, requested together and added
+// in the order of k.
+constexpr int kMaxSplits = 4;
+__device__ __forceinline__ float4 sum_of_splits(uint32_t at, int splits) {
+  float4 v[kMaxSplits];
+#pragma unroll
+  for (int r = 0; r < kMaxSplits; ++r)
+    if (r < splits) v[r] = ld_cluster_f32x4(map_to_cta(at, r));
+  float4 sum = v[0];
+#pragma unroll
+  for (int r = 1; r < kMaxSplits; ++r)
+    if (r < splits) { sum.x += v[r].x; sum.y += v[r].y; sum.z += v[r].z; sum.w += v[r].w; }
+  return sum;
 }
 
 // One tile: rows [row0, row0 + ntok) of group g against weight rows [128 nb, 128 nb + 128).
@@ -111,7 +153,7 @@ __device__ __forceinline__ GemmTile tile_at(const Fp8GemmArgs &p, const int *s_t
 
 template <int kTok>
 __global__ void __launch_bounds__(GemmShape<kTok>::kThreads, 1)
-fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const Fp8GemmArgs p) {
+fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const Fp8GemmArgs p, const int wide_out) {
   using S = GemmShape<kTok>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ int s_tiles[kMaxGemmGroups + 1];   // token tiles of the groups before g
@@ -123,16 +165,19 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
   auto full = [&](int s) { return bars + 8u * s; };
   auto empty = [&](int s) { return bars + 8u * (S::kStages + s); };
   auto dfull = [&](int d) { return bars + 8u * (2 * S::kStages + d); };
-  auto dempty = [&](int d) { return bars + 8u * (2 * S::kStages + kAccBufs + d); };
-  auto sfull = [&](int s) { return bars + 8u * (2 * S::kStages + 2 * kAccBufs + s); };
-  auto sempty = [&](int s) { return bars + 8u * (2 * S::kStages + 2 * kAccBufs + kScaleSlots + s); };
+  auto dempty = [&](int d) { return bars + 8u * (2 * S::kStages + S::kAccBufs + d); };
+  auto sfull = [&](int s) { return bars + 8u * (2 * S::kStages + 2 * S::kAccBufs + s); };
+  auto sempty = [&](int s) { return bars + 8u * (2 * S::kStages + 2 * S::kAccBufs + kScaleSlots + s); };
+  auto pfull = [&](int i) { return bars + 8u * (2 * S::kStages + 2 * S::kAccBufs + 2 * kScaleSlots + i); };
+  auto pempty = [&](int i) { return bars + 8u * (2 * S::kStages + 2 * S::kAccBufs + 2 * kScaleSlots + 2 + i); };
   constexpr int kCopyWarp = S::kEpiWarps, kMmaWarp = kCopyWarp + 1, kScaleWarp = kCopyWarp + 2;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::kStages; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
-    for (int d = 0; d < kAccBufs; ++d) { mbar_init(dfull(d), 1); mbar_init(dempty(d), S::kEpiWarps); }
+    for (int d = 0; d < S::kAccBufs; ++d) { mbar_init(dfull(d), 1); mbar_init(dempty(d), S::kEpiWarps); }
     for (int s = 0; s < kScaleSlots; ++s) { mbar_init(sfull(s), 1); mbar_init(sempty(s), S::kEpiWarps); }
+    for (int i = 0; i < 2; ++i) { mbar_init(pfull(i), 1); mbar_init(pempty(i), S::kEpiWarps); }
     s_abort = 0u;
     fence_mbar_init();
   }
@@ -186,11 +231,10 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
     const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
     const uint64_t desc = smem_desc_sw128(0);
     for (int it = blockIdx.x; ok && it < n_items; it += stride) {
-      const GemmTile t = tile_of(it);
-      const uint32_t idesc = idesc_e4m3(kScaleBlock, (t.ntok + 15) / 16 * 16);
+      const uint32_t idesc = __shfl_sync(0xffffffffu, idesc_e4m3(kScaleBlock, (tile_of(it).ntok + 15) / 16 * 16), 0);   // uniform
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait_warp(dempty(d), dpar, abort_flag, p.status, ST_WAIT_DEMPTY)) { ok = false; break; }
         if (!mbar_wait_warp(full(s), par, abort_flag, p.status, ST_WAIT_FULL)) { ok = false; break; }
+        if (!mbar_wait_warp(dempty(d), dpar, abort_flag, p.status, ST_WAIT_DEMPTY)) { ok = false; break; }
         tc_fence_after();
         if (elect_one()) {
           const uint32_t stage = ring + s * S::kStageBytes, acc = tm + d * S::kBufCols;
@@ -202,97 +246,184 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
         }
         __syncwarp();
         if (++s == S::kStages) { s = 0; par ^= 1u; }
-        if (++d == kAccBufs) { d = 0; dpar ^= 1u; }
+        if (++d == S::kAccBufs) { d = 0; dpar ^= 1u; }
       }
     }
   } else if (warp == kScaleWarp) {
-    // ---- scales of the tile's tokens times the block's own, one slot per block of k; four blocks are fetched together
-    constexpr int kPer = kTok < 32 ? 1 : kTok / 32, kAhead = 4;
-    uint32_t s = 0, par = 1u;
+    // ---- scales of the tile's tokens times the block's own, kScaleBlocks blocks of k to a slot
+    constexpr int kPer = kTok < 32 ? 1 : kTok / 32, kPass = kPer < 4 ? kPer : 4;   // tokens of a lane; of these, fetched together
+    uint32_t s = 0, par = 1u, plan = 0, ppar = 1u;
     float *slots = reinterpret_cast<float *>(ring_ptr + S::kScaleOff);
     for (int it = blockIdx.x; ok && it < n_items; it += stride) {
       const GemmTile t = tile_of(it);
+      float bias[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int n = t.nb * kScaleBlock + 32 * i + lane;
+        bias[i] = p.bias != nullptr && n < p.n ? __bfloat162float(p.bias[static_cast<size_t>(t.g) * p.n + n]) : 0.f;
+      }
+      if (!mbar_wait_warp(pempty(plan), ppar, abort_flag, p.status, ST_WAIT_AFREE)) { ok = false; break; }
+      uint8_t *at = ring_ptr + S::kPlanOff + plan * S::kPlanBytes;
+      if (lane == 0) *reinterpret_cast<GemmTile *>(at) = t;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) reinterpret_cast<float *>(at + 16)[32 * i + lane] = bias[i];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(pfull(plan));
+      if (plan ^= 1u; plan == 0) ppar ^= 1u;
       const float *sb = p.sb + (static_cast<size_t>(t.g) * n_nb + t.nb) * p.n_kb;
-      for (int kq = kb0; ok && kq < kb1; kq += kAhead) {
-        float v[kAhead][kPer];
+      for (int k0 = kb0; ok && k0 < kb1; k0 += kScaleBlocks) {
+        const float b = lane < kScaleBlocks && k0 + lane < kb1 ? sb[k0 + lane] : 0.f;
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
-          const int kb = min(kq + j, kb1 - 1);
-          const float b = sb[kb];
+        for (int i0 = 0; i0 < kPer; i0 += kPass) {
+          float v[kPass][kScaleBlocks];
 #pragma unroll
-          for (int i = 0; i < kPer; ++i) {
-            const int tok = lane + 32 * i;
-            v[j][i] = tok < t.ntok ? p.sa[static_cast<size_t>(t.row0 + tok) * p.ld_sa + kb] * b : 0.f;
+          for (int i = 0; i < kPass; ++i) {
+            const int tok = lane + 32 * (i0 + i);
+            const float *sa = p.sa + static_cast<size_t>(t.row0 + tok) * p.ld_sa + k0;
+#pragma unroll
+            for (int j = 0; j < kScaleBlocks; ++j) v[i][j] = tok < t.ntok && k0 + j < kb1 ? sa[j] : 0.f;
+          }
+          if (i0 == 0 && !mbar_wait_warp(sempty(s), par, abort_flag, p.status, ST_WAIT_AFREE)) { ok = false; break; }
+#pragma unroll
+          for (int j = 0; j < kScaleBlocks; ++j) {
+            const float f = __shfl_sync(0xffffffffu, b, j);
+#pragma unroll
+            for (int i = 0; i < kPass; ++i)
+              if (lane + 32 * (i0 + i) < kTok) slots[(s * kScaleBlocks + j) * kTok + lane + 32 * (i0 + i)] = v[i][j] * f;
           }
         }
-#pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
-          if (!ok || kq + j >= kb1) break;
-          if (!mbar_wait_warp(sempty(s), par, abort_flag, p.status, ST_WAIT_AFREE)) { ok = false; break; }
-#pragma unroll
-          for (int i = 0; i < kPer; ++i)
-            if (lane + 32 * i < kTok) slots[s * kTok + lane + 32 * i] = v[j][i];
-          __syncwarp();
-          if (lane == 0) mbar_arrive(sfull(s));
-          if (++s == kScaleSlots) { s = 0; par ^= 1u; }
-        }
+        if (!ok) break;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(sfull(s));
+        if (++s == kScaleSlots) { s = 0; par ^= 1u; }
       }
     }
   } else {
-    // ---- sums over the blocks: warp w holds weight rows 32 (w % 4).. (a lane each) of kCols token columns
-    const int quad = warp & 3, col0 = (warp >> 2) * S::kCols;
+    // ---- sums over the blocks: warp w has weight rows 32 (w % 4) .. + 31 and kCols token columns, as fragments: of the columns
+    // 8 j .. 8 j + 7 and rows 16 h + 8 i + lane / 4 the pair 2 (lane % 4), + 1 is acc[j][h][i]
+    const int quad = warp & 3, col0 = (warp >> 2) * S::kCols, pair0 = 2 * (lane & 3);
     const uint32_t lane_field = static_cast<uint32_t>(quad * 32) << 16;
-    const float4 *slots = reinterpret_cast<const float4 *>(ring_ptr + S::kScaleOff);
-    uint32_t d = 0, dpar = 0, s = 0, spar = 0;
+    const float *slots = reinterpret_cast<const float *>(ring_ptr + S::kScaleOff) + col0 + pair0;
+    uint32_t d = 0, dpar = 0, s = 0, spar = 0, plan = 0, ppar = 0;
     for (int it = blockIdx.x; ok && it < n_items; it += stride) {
-      const GemmTile t = tile_of(it);
-      const int nrow = t.nb * kScaleBlock + quad * 32 + lane;
-      float acc[S::kCols];
+      if (!mbar_wait_warp(pfull(plan), ppar, abort_flag, p.status, ST_WAIT_AREADY)) { ok = false; break; }
+      const uint8_t *at = ring_ptr + S::kPlanOff + plan * S::kPlanBytes;
+      const GemmTile t = *reinterpret_cast<const GemmTile *>(at);
+      uint64_t acc[S::kCols / 8][2][2];
 #pragma unroll
-      for (int c = 0; c < S::kCols; ++c) acc[c] = 0.f;
+      for (int j = 0; j < S::kCols / 8; ++j) acc[j][0][0] = acc[j][0][1] = acc[j][1][0] = acc[j][1][1] = 0ull;
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait_warp(sfull(s), spar, abort_flag, p.status, ST_WAIT_AREADY)) { ok = false; break; }
+        const int kq = (kb - kb0) % kScaleBlocks;
+        if (kq == 0 && !mbar_wait_warp(sfull(s), spar, abort_flag, p.status, ST_WAIT_AREADY)) { ok = false; break; }
         if (!mbar_wait_warp(dfull(d), dpar, abort_flag, p.status, ST_WAIT_DFULL)) { ok = false; break; }
         tc_fence_after();
         const uint32_t src = tmem + lane_field + d * S::kBufCols + col0;
-        uint32_t v[S::kCols / 16][16];
+        const float *f = slots + (s * kScaleBlocks + kq) * kTok;
 #pragma unroll
-        for (int c = 0; c < S::kCols / 16; ++c)
-          if (col0 + 16 * c < t.ntok) tmem_ld16(src + 16 * c, v[c]);
-        tmem_wait_ld();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(dempty(d));
+        for (int c = 0; c < S::kCols; c += S::kChunk) {
+          constexpr int kLd = S::kChunk < 32 ? 16 : 32;   // columns of a load
+          uint32_t v[S::kChunk / kLd][2][kLd / 2];
 #pragma unroll
-        for (int c = 0; c < S::kCols / 16; ++c)
-          if (col0 + 16 * c < t.ntok) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float4 f = slots[(s * kTok + col0 + 16 * c) / 4 + i];
-              float *a = acc + 16 * c + 4 * i;
-              a[0] = fmaf(__uint_as_float(v[c][4 * i]), f.x, a[0]);
-              a[1] = fmaf(__uint_as_float(v[c][4 * i + 1]), f.y, a[1]);
-              a[2] = fmaf(__uint_as_float(v[c][4 * i + 2]), f.z, a[2]);
-              a[3] = fmaf(__uint_as_float(v[c][4 * i + 3]), f.w, a[3]);
+          for (int l = 0; l < S::kChunk / kLd; ++l)
+            if (col0 + c + l * kLd < t.ntok) {
+              tmem_ld_frag(src + c + l * kLd, v[l][0]);
+              tmem_ld_frag(src + c + l * kLd + (16u << 16), v[l][1]);
             }
+          tmem_wait_ld();
+          if (c + S::kChunk == S::kCols) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(dempty(d));
           }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(sempty(s));
-        if (++d == kAccBufs) { d = 0; dpar ^= 1u; }
-        if (++s == kScaleSlots) { s = 0; spar ^= 1u; }
+#pragma unroll
+          for (int l = 0; l < S::kChunk / kLd; ++l)
+            if (col0 + c + l * kLd < t.ntok) {
+#pragma unroll
+              for (int j = 0; j < kLd / 8; ++j) {
+                const uint64_t f2 = *reinterpret_cast<const uint64_t *>(f + c + l * kLd + 8 * j);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                  for (int i = 0; i < 2; ++i) fma_f32x2(acc[(c + l * kLd) / 8 + j][h][i], v[l][h][4 * j + 2 * i], v[l][h][4 * j + 2 * i + 1], f2);
+              }
+            }
+        }
+        if (kq == kScaleBlocks - 1 || kb + 1 == kb1) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(sempty(s));
+          if (++s == kScaleSlots) { s = 0; spar ^= 1u; }
+        }
+        if (++d == S::kAccBufs) { d = 0; dpar ^= 1u; }
       }
       if (!ok) break;
+      const int n_w = t.nb * kScaleBlock + quad * 32;   // first weight row of the warp
+      auto value = [&](int j, int h, int i, int c) { return __uint_as_float(static_cast<uint32_t>(acc[j][h][i] >> (32 * c))); };
       if (p.splits > 1) {
         // every MMA of this CTA is complete: the ring takes the partial tile, [token][weight row]
         float *part = reinterpret_cast<float *>(ring_ptr);
 #pragma unroll
-        for (int c = 0; c < S::kCols; ++c)
-          if (col0 + c < t.ntok) part[(col0 + c) * kScaleBlock + quad * 32 + lane] = acc[c];
-      } else if (nrow < p.n) {
-        const float b = p.bias != nullptr ? __bfloat162float(p.bias[static_cast<size_t>(t.g) * p.n + nrow]) : 0.f;
+        for (int j = 0; j < S::kCols / 8; ++j)
+          if (col0 + 8 * j < t.ntok) {
 #pragma unroll
-        for (int c = 0; c < S::kCols; ++c)
-          if (col0 + c < t.ntok) store_out(p, static_cast<size_t>(t.row0 + col0 + c) * p.ld_out + nrow, acc[c] + b);
+            for (int e = 0; e < 8; ++e) {
+              const int h = e >> 2, i = (e >> 1) & 1, c = e & 1;
+              part[(col0 + 8 * j + pair0 + c) * S::kPartPitch + quad * 32 + 16 * h + 8 * i + (lane >> 2)] = value(j, h, i, c);
+            }
+          }
+        break;   // a split CTA has one tile
+      }
+      float b[2][2];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) b[e >> 1][e & 1] = reinterpret_cast<const float *>(at + 16)[quad * 32 + 8 * e + (lane >> 2)];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(pempty(plan));
+      if (plan ^= 1u; plan == 0) ppar ^= 1u;
+      if (wide_out) {
+        // 16-bit outputs: blocks of 8 tokens x 32 weight rows are transposed in shared memory and leave as 16 bytes a lane
+        const uint32_t stage = ring + S::kOutOff + warp * S::kOutWarp;
+        const uint32_t st_at = stage + (lane & 7) * S::kOutPitch + (lane >> 3) * 16, ld_at = stage + (lane >> 2) * S::kOutPitch + (lane & 3) * 16;
+        const int n = n_w + (lane & 3) * 8, ntok = t.ntok - col0;
+        uint16_t *dst = static_cast<uint16_t *>(p.out) + static_cast<size_t>(t.row0 + col0 + (lane >> 2)) * p.ld_out + n;
+#pragma unroll
+        for (int j0 = 0; j0 < S::kCols / 8; j0 += S::kOutCols / 8) {
+          if (8 * j0 >= ntok) break;
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < S::kOutCols / 8; ++j) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int h = e >> 1, i = e & 1;
+              const float x = value(j0 + j, h, i, 0) + b[h][i], y = value(j0 + j, h, i, 1) + b[h][i];
+              w[e] = p.out_dtype == MOE_BF16 ? pack2<__nv_bfloat16>(x, y) : pack2<__half>(x, y);
+            }
+            stmatrix_trans_x4(st_at + j * 8 * S::kOutPitch, w[0], w[1], w[2], w[3]);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < S::kOutCols / 8; ++j, dst += 8 * p.ld_out) {
+            if (8 * (j0 + j) + (lane >> 2) >= ntok || n >= p.n) continue;
+            uint32_t o[4];
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]) : "r"(ld_at + j * 8 * S::kOutPitch) : "memory");
+            if (n + 8 <= p.n) {
+              *reinterpret_cast<uint4 *>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                if (n + e < p.n) dst[e] = static_cast<uint16_t>(o[e / 2] >> (16 * (e & 1)));
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < S::kCols / 8; ++j) {
+          if (col0 + 8 * j >= t.ntok) break;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int h = e >> 2, i = (e >> 1) & 1, c = e & 1, tok = col0 + 8 * j + pair0 + c, n = n_w + 16 * h + 8 * i + (lane >> 2);
+            if (tok < t.ntok && n < p.n) store_out(p, static_cast<size_t>(t.row0 + tok) * p.ld_out + n, value(j, h, i, c) + b[h][i]);
+          }
+        }
       }
     }
   }
@@ -305,14 +436,14 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
       const GemmTile t = tile_of(it);
       const uint32_t base = smem_u32(ring_ptr);
       const int mine = (t.ntok - split + p.splits - 1) / p.splits;
-      for (int e = threadIdx.x; e < mine * kScaleBlock; e += S::kThreads) {
-        const int tok = split + e / kScaleBlock * p.splits, r = e % kScaleBlock, nrow = t.nb * kScaleBlock + r;
-        float sum = 0.f;
-        for (int c = 0; c < p.splits; ++c) sum += ld_cluster_f32(map_to_cta(base + 4u * (tok * kScaleBlock + r), c));
-        if (nrow < p.n) {
-          const float b = p.bias != nullptr ? __bfloat162float(p.bias[static_cast<size_t>(t.g) * p.n + nrow]) : 0.f;
-          store_out(p, static_cast<size_t>(t.row0 + tok) * p.ld_out + nrow, sum + b);
-        }
+      for (int e = threadIdx.x; e < mine * (kScaleBlock / 4); e += S::kThreads) {
+        const int tok = split + e / (kScaleBlock / 4) * p.splits, r = e % (kScaleBlock / 4) * 4, n = t.nb * kScaleBlock + r;
+        const float4 sum = sum_of_splits(base + 4u * (tok * S::kPartPitch + r), p.splits);
+        const float o[4] = {sum.x, sum.y, sum.z, sum.w};
+        const size_t at = static_cast<size_t>(t.row0 + tok) * p.ld_out + n;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (n + i < p.n) store_out(p, at + i, o[i] + (p.bias != nullptr ? __bfloat162float(p.bias[static_cast<size_t>(t.g) * p.n + n + i]) : 0.f));
       }
     }
     cluster_sync_all();   // no CTA leaves while another may still read its part
@@ -329,51 +460,35 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
 }
 
 // ---------------------------------------------------------------------------
-// Many rows per group: a pair of CTAs on 256 token rows x 256 weight rows.  Here the token rows are the M operand (a lane of
-// tensor memory each, 128 in either CTA), so that sa * sb is one number per thread and block; each CTA holds half of the
-// weight rows, which the pair's tensor cores share.
+// Many rows per group: 128 token rows x 256 weight rows.  Here the token rows are the M operand (a lane of tensor memory each),
+// so that sa * sb is one number per thread and block.
 // ---------------------------------------------------------------------------
-constexpr int kPairTok = 256, kPairN = 256;
-constexpr int kPairTile = 128 * kScaleBlock;     // bytes of 128 rows of a block of k: the CTA's token rows, and its weight rows
-constexpr int kPairStage = 2 * kPairTile, kPairStages = 4, kPairAccBufs = 2;
-constexpr int kPairEpiWarps = 8, kPairThreads = (kPairEpiWarps + 4) * 32;
-constexpr int kPairCols = kPairN / (kPairEpiWarps / 4);    // accumulator columns of a warp: one scale block of the weights
-constexpr int kOutBox = 32 * 128, kOutWarp = 2 * kOutBox;  // outputs on their way out: 32 rows of 128 bytes, two a warp
-constexpr int kPairOutOff = kPairStages * kPairStage;
-constexpr int kPairBiasOff = kPairOutOff + kPairEpiWarps * kOutWarp;
-constexpr int kScaleBlocks = 8, kPairScaleSlots = 2;       // blocks of k whose scales are handed over at once
-constexpr int kPairScaleOff = kPairBiasOff + 2 * kPairN * 4;           // [slot][half][block][128 rows]
-constexpr int kPairScaleSlot = 2 * kScaleBlocks * 128;                 // floats
-constexpr int kPairBarOff = kPairScaleOff + kPairScaleSlots * kPairScaleSlot * 4;
-constexpr int kPairBars = 2 * kPairStages + 4 * kPairAccBufs + 2 * kPairScaleSlots + 4;
-constexpr int kPairSmem = kPairBarOff + 8 * kPairBars + 1024;
-static_assert(kPairCols == kScaleBlock, "one sb per warp and block of k");
-static_assert(kPairSmem + 8 * 1024 <= 227 * 1024, "shared memory");
+constexpr int kWideTok = 128, kWideN = 256;
+constexpr int kWideTile = kWideTok * kScaleBlock;                       // bytes of the token rows of a block of k
+constexpr int kWideStage = kWideTile + kWideN * kScaleBlock, kWideStages = 3, kWideAccBufs = 2;
+constexpr int kWideEpiWarps = 8, kWideThreads = (kWideEpiWarps + 3) * 32;
+constexpr int kWidePart = kWideN + 4;                      // floats of a row of a split's partial tile: no bank conflicts
+constexpr int kWideCols = kWideN / (kWideEpiWarps / 4);
+constexpr int kOutBox = 32 * 128;                          // outputs of a warp on their way out: 32 rows of 128 bytes
+constexpr int kWideOutOff = kWideStages * kWideStage;
+constexpr int kWideBiasOff = kWideOutOff + kWideEpiWarps * kOutBox;
+constexpr int kWideScaleOff = kWideBiasOff + 2 * kWideN * 4;
+constexpr int kWideScaleSlot = 2 * kScaleBlocks * 128;
+constexpr int kWideBarOff = kWideScaleOff + kScaleSlots * kWideScaleSlot * 4;
+constexpr int kWideBars = 2 * kWideStages + 2 * kWideAccBufs + 2 * kScaleSlots + 4;
+constexpr int kWideSmem = kWideBarOff + 8 * kWideBars + 1024;
+static_assert(kWideCols == kScaleBlock, "one sb per warp and block of k");
+static_assert(kWideTok * kWidePart * 4 <= kWideStages * kWideStage, "a split's partial tile reuses the ring");
+static_assert(kWideSmem + 4608 <= 227 * 1024, "shared memory");
 
-__device__ __forceinline__ void fma_f32x2(uint64_t &acc, uint32_t lo, uint32_t hi, uint64_t f) {
-  asm("{\n\t.reg .b64 v;\n\tmov.b64 v, {%1, %2};\n\tfma.rn.f32x2 %0, v, %3, %0;\n\t}" : "+l"(acc) : "r"(lo), "r"(hi), "l"(f));
-}
-
-template <class T>
-__device__ __forceinline__ uint32_t pack2(float a, float b);
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t *>(&h);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t *>(&h);
-}
-// What the copy engine would do with two boxes of staged outputs (128-byte swizzle), by a warp: rows [0, rows) to output rows
+// What the copy engine would do with a box of staged outputs (128-byte swizzle), by a warp: rows [0, rows) to output rows
 // row0.. and columns n..; 16 bytes a lane where the output is aligned for it, else an element.
-__device__ __forceinline__ void copy_rows(const Fp8GemmArgs &p, const uint8_t *boxes, int row0, int rows, int n, int box_cols) {
+__device__ __forceinline__ void copy_box(const Fp8GemmArgs &p, const uint8_t *box, int row0, int rows, int n) {
   const int lane = threadIdx.x & 31, size = p.out_dtype == MOE_F32 ? 4 : 2, per = 16 / size;
   const bool wide = (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0 && p.ld_out % per == 0;
-  for (int i = lane; i < rows * 16; i += 32) {   // (row, box, 16-byte piece)
-    const int r = i / 16, box = i / 8 % 2, piece = i % 8, col = n + box * box_cols + piece * per;
-    const uint4 v = *reinterpret_cast<const uint4 *>(boxes + box * kOutBox + r * 128 + ((piece ^ (r & 7)) << 4));
+  for (int i = lane; i < rows * 8; i += 32) {   // (row, 16-byte piece)
+    const int r = i / 8, piece = i % 8, col = n + piece * per;
+    const uint4 v = *reinterpret_cast<const uint4 *>(box + r * 128 + ((piece ^ (r & 7)) << 4));
     const size_t at = static_cast<size_t>(row0 + r) * p.ld_out + col;
     if (wide && col + per <= p.n) {
       *reinterpret_cast<uint4 *>(static_cast<uint8_t *>(p.out) + at * size) = v;
@@ -388,43 +503,42 @@ __device__ __forceinline__ void copy_rows(const Fp8GemmArgs &p, const uint8_t *b
   }
 }
 
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
-fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_out,
+// kSplit: a cluster of p.splits CTAs, blockIdx.y of them, shares the reduction of one tile.
+template <bool kSplit>
+__global__ void __launch_bounds__(kWideThreads, 1)
+fp8_gemm_wide_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_out,
                      const Fp8GemmArgs p, const int tiled_out) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ int s_tiles[kMaxGemmGroups + 1];
   __shared__ uint32_t s_tmem, s_abort;
   volatile uint32_t *abort_flag = &s_abort;
   const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  float *s_bias = reinterpret_cast<float *>(smem_raw + (ring - smem_u32(smem_raw)) + kPairBiasOff);   // [2][kPairN]
-  float *s_scales = reinterpret_cast<float *>(smem_raw + (ring - smem_u32(smem_raw)) + kPairScaleOff);
-  const uint32_t bars = ring + kPairBarOff;
+  float *s_bias = reinterpret_cast<float *>(smem_raw + (ring - smem_u32(smem_raw)) + kWideBiasOff);   // [2][kWideN]
+  float *s_scales = reinterpret_cast<float *>(smem_raw + (ring - smem_u32(smem_raw)) + kWideScaleOff);
+  const uint32_t bars = ring + kWideBarOff;
   auto full = [&](int s) { return bars + 8u * s; };
-  auto empty = [&](int s) { return bars + 8u * (kPairStages + s); };
-  auto dfull = [&](int h, int d) { return bars + 8u * (2 * kPairStages + kPairAccBufs * h + d); };
-  auto dempty = [&](int h, int d) { return bars + 8u * (2 * kPairStages + kPairAccBufs * (2 + h) + d); };
-  constexpr int kSideBars = 2 * kPairStages + 4 * kPairAccBufs;
+  auto empty = [&](int s) { return bars + 8u * (kWideStages + s); };
+  auto dfull = [&](int d) { return bars + 8u * (2 * kWideStages + d); };
+  auto dempty = [&](int d) { return bars + 8u * (2 * kWideStages + kWideAccBufs + d); };
+  constexpr int kSideBars = 2 * kWideStages + 2 * kWideAccBufs;
   auto bfull = [&](int i) { return bars + 8u * (kSideBars + i); };
   auto bempty = [&](int i) { return bars + 8u * (kSideBars + 2 + i); };
   auto sfull = [&](int i) { return bars + 8u * (kSideBars + 4 + i); };
-  auto sempty = [&](int i) { return bars + 8u * (kSideBars + 4 + kPairScaleSlots + i); };
-  constexpr int kCopyWarp = kPairEpiWarps, kSideWarp = kCopyWarp + 1, kMmaWarp = kCopyWarp + 2;   // two MMA warps
+  auto sempty = [&](int i) { return bars + 8u * (kSideBars + 4 + kScaleSlots + i); };
+  constexpr int kCopyWarp = kWideEpiWarps, kSideWarp = kCopyWarp + 1, kMmaWarp = kCopyWarp + 2;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = static_cast<int>(cluster_ctarank());   // 0 issues the MMAs of the pair
 
   if (threadIdx.x == 0) {
-    // full and dempty are used in the even CTA only: the copies of both CTAs, the epilogue warps of both
-    for (int s = 0; s < kPairStages; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 2); }
-    for (int h = 0; h < 2; ++h)
-      for (int d = 0; d < kPairAccBufs; ++d) { mbar_init(dfull(h, d), 1); mbar_init(dempty(h, d), kPairEpiWarps); }   // half of either CTA's
-    for (int i = 0; i < 2; ++i) { mbar_init(bfull(i), 1); mbar_init(bempty(i), kPairEpiWarps); }
-    for (int i = 0; i < kPairScaleSlots; ++i) { mbar_init(sfull(i), 1); mbar_init(sempty(i), kPairEpiWarps); }
+    for (int s = 0; s < kWideStages; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
+    for (int d = 0; d < kWideAccBufs; ++d) { mbar_init(dfull(d), 1); mbar_init(dempty(d), kWideEpiWarps); }
+    for (int i = 0; i < 2; ++i) { mbar_init(bfull(i), 1); mbar_init(bempty(i), kWideEpiWarps); }
+    for (int i = 0; i < kScaleSlots; ++i) { mbar_init(sfull(i), 1); mbar_init(sempty(i), kWideEpiWarps); }
     s_abort = 0u;
     fence_mbar_init();
   }
   if (warp == kMmaWarp) {
-    tmem_alloc_pair(smem_u32(&s_tmem), kPairAccBufs * kPairN);
-    tmem_relinquish_pair();
+    tmem_alloc(smem_u32(&s_tmem), kWideAccBufs * kWideN);
+    tmem_relinquish();
   }
   if (warp == kCopyWarp && lane == 0) {
     prefetch_tensormap(&tm_a);
@@ -433,57 +547,55 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
   }
   grid_dep_sync();   // from here on what other kernels wrote is read
   tc_fence_before();
-  count_tiles<kPairTok>(p, s_tiles);
-  cluster_sync_all();   // the peer's barriers exist before anything arrives on them
+  count_tiles<kWideTok>(p, s_tiles);
   tc_fence_after();
   const uint32_t tmem = s_tmem;
-  const int n_nb = (p.n + kPairN - 1) / kPairN, n_sb = (p.n + kScaleBlock - 1) / kScaleBlock;
+  const int n_nb = (p.n + kWideN - 1) / kWideN, n_sb = (p.n + kScaleBlock - 1) / kScaleBlock;
   const int n_items = s_tiles[p.n_groups] * n_nb;
-  const int first = blockIdx.x >> 1, stride = gridDim.x >> 1;
+  const int first = blockIdx.x, stride = kSplit ? n_items : gridDim.x;   // a split CTA takes one tile
+  const int split = kSplit ? static_cast<int>(blockIdx.y) : 0;
+  const int kb0 = kSplit ? static_cast<int>(static_cast<long long>(p.n_kb) * split / p.splits) : 0;
+  const int kb1 = kSplit ? static_cast<int>(static_cast<long long>(p.n_kb) * (split + 1) / p.splits) : p.n_kb;
   bool ok = true;
 
-  if (warp >= kPairEpiWarps) {
+  if (warp >= kWideEpiWarps) {
     if (warp == kCopyWarp) {
       uint32_t s = 0, par = 1u;
-      const uint32_t full0 = map_to_cta(full(0), 0);
       for (int it = first; ok && it < n_items; it += stride) {
         const GemmTile t = tile_at(p, s_tiles, it, n_nb);
-        for (int kb = 0; kb < p.n_kb; ++kb) {
-          if (!mbar_wait_warp<Wait::kClusterRelaxed>(empty(s), par, abort_flag, p.status, ST_WAIT_EMPTY)) { ok = false; break; }
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait_warp(empty(s), par, abort_flag, p.status, ST_WAIT_EMPTY)) { ok = false; break; }
           if (elect_one()) {
-            const uint32_t stage = ring + s * kPairStage;
-            if (rank == 0) mbar_arrive_expect_tx(full(s), 2 * kPairStage);
-            tma_load_2d_pair(stage, &tm_a, kb * kScaleBlock, t.row0 + 128 * rank, full0 + 8u * s);
-            for (int h = 0; h < 2; ++h)   // 64 of the 128 weight rows of either half
-              tma_load_3d_pair(stage + kPairTile + h * (kPairTile / 2), &tm_b, kb * kScaleBlock, t.nb * kPairN + 128 * h + 64 * rank, t.g, full0 + 8u * s);
+            const uint32_t stage = ring + s * kWideStage;
+            mbar_arrive_expect_tx(full(s), kWideStage);
+            tma_load_2d(stage, &tm_a, kb * kScaleBlock, t.row0, full(s));
+            tma_load_3d(stage + kWideTile, &tm_b, kb * kScaleBlock, t.nb * kWideN, t.g, full(s));
           }
           __syncwarp();
-          if (++s == kPairStages) { s = 0; par ^= 1u; }
+          if (++s == kWideStages) { s = 0; par ^= 1u; }
         }
       }
-    } else if (warp >= kMmaWarp && rank == 0) {
-      // ---- MMA: a warp for either half of the columns, with accumulators of its own
-      const int half = warp - kMmaWarp;
+    } else if (warp == kMmaWarp) {
       uint32_t s = 0, par = 0, d = 0, dpar = 1u;
-      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0) + half * kPairAccBufs * kPairCols;
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
       const uint64_t desc = smem_desc_sw128(0);
-      constexpr uint32_t idesc = idesc_e4m3(256, kPairCols);
+      constexpr uint32_t idesc = idesc_e4m3(128, kWideN);
       for (int it = first; ok && it < n_items; it += stride) {
-        for (int kb = 0; kb < p.n_kb; ++kb) {
-          if (!mbar_wait_warp<Wait::kCluster>(full(s), par, abort_flag, p.status, ST_WAIT_FULL)) { ok = false; break; }
-          if (!mbar_wait_warp<Wait::kClusterRelaxed>(dempty(half, d), dpar, abort_flag, p.status, ST_WAIT_DEMPTY)) { ok = false; break; }
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait_warp(full(s), par, abort_flag, p.status, ST_WAIT_FULL)) { ok = false; break; }
+          if (!mbar_wait_warp(dempty(d), dpar, abort_flag, p.status, ST_WAIT_DEMPTY)) { ok = false; break; }
           tc_fence_after();
           if (elect_one()) {
-            const uint32_t stage = ring + s * kPairStage, acc = tm + d * kPairCols;
-            const uint64_t xd = desc | (stage >> 4), wd = desc | ((stage + kPairTile + half * (kPairTile / 2)) >> 4);
+            const uint32_t stage = ring + s * kWideStage, acc = tm + d * kWideN;
+            const uint64_t xd = desc | (stage >> 4), wd = desc | ((stage + kWideTile) >> 4);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) mma_f8_pair(acc, xd + 2 * i, wd + 2 * i, idesc, i > 0);
-            mma_commit_pair(dfull(half, d));
-            mma_commit_pair(empty(s));
+            for (int i = 0; i < 4; ++i) mma_f8(acc, xd + 2 * i, wd + 2 * i, idesc, i > 0);
+            mma_commit(dfull(d));
+            mma_commit(empty(s));
           }
           __syncwarp();
-          if (++s == kPairStages) { s = 0; par ^= 1u; }
-          if (++d == kPairAccBufs) { d = 0; dpar ^= 1u; }
+          if (++s == kWideStages) { s = 0; par ^= 1u; }
+          if (++d == kWideAccBufs) { d = 0; dpar ^= 1u; }
         }
       }
     }
@@ -494,24 +606,24 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
         const GemmTile t = tile_at(p, s_tiles, it, n_nb);
         // rows and weight blocks that do not exist take the scales of the last one: their sums go nowhere
         const float *sb0 = p.sb + (static_cast<size_t>(t.g) * n_sb + 2 * t.nb) * p.n_kb, *sb1 = 2 * t.nb + 1 < n_sb ? sb0 + p.n_kb : sb0;
-        float bias[kPairN / 32];
+        float bias[kWideN / 32];
 #pragma unroll
-        for (int i = 0; i < kPairN / 32; ++i) {
-          const int n = t.nb * kPairN + 32 * i + lane;
+        for (int i = 0; i < kWideN / 32; ++i) {
+          const int n = t.nb * kWideN + 32 * i + lane;
           bias[i] = p.bias != nullptr && n < p.n ? __bfloat162float(p.bias[static_cast<size_t>(t.g) * p.n + n]) : 0.f;
         }
-        for (int k0 = 0; ok && k0 < p.n_kb; k0 += kScaleBlocks) {
-          const bool mine = lane < kScaleBlocks && k0 + lane < p.n_kb;
+        for (int k0 = kb0; ok && k0 < kb1; k0 += kScaleBlocks) {
+          const bool mine = lane < kScaleBlocks && k0 + lane < kb1;
           const float b0 = mine ? sb0[k0 + lane] : 0.f, b1 = mine ? sb1[k0 + lane] : 0.f;
           float v[4][kScaleBlocks];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float *sa = p.sa + static_cast<size_t>(t.row0 + min(128 * rank + 32 * r + lane, t.ntok - 1)) * p.ld_sa + k0;
+            const float *sa = p.sa + static_cast<size_t>(t.row0 + min(32 * r + lane, t.ntok - 1)) * p.ld_sa + k0;
 #pragma unroll
-            for (int j = 0; j < kScaleBlocks; ++j) v[r][j] = k0 + j < p.n_kb ? sa[j] : 0.f;
+            for (int j = 0; j < kScaleBlocks; ++j) v[r][j] = k0 + j < kb1 ? sa[j] : 0.f;
           }
           if (!mbar_wait_warp(sempty(s), par, abort_flag, p.status, ST_WAIT_AFREE)) { ok = false; break; }
-          float *dst = s_scales + s * kPairScaleSlot + lane;
+          float *dst = s_scales + s * kWideScaleSlot + lane;
 #pragma unroll
           for (int j = 0; j < kScaleBlocks; ++j) {
             const float f0 = __shfl_sync(0xffffffffu, b0, j), f1 = __shfl_sync(0xffffffffu, b1, j);
@@ -523,11 +635,11 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(sfull(s));
-          if (++s == kPairScaleSlots) { s = 0; par ^= 1u; }
+          if (++s == kScaleSlots) { s = 0; par ^= 1u; }
         }
         if (!ok || !mbar_wait_warp(bempty(buf), bpar, abort_flag, p.status, ST_WAIT_AFREE)) { ok = false; break; }
 #pragma unroll
-        for (int i = 0; i < kPairN / 32; ++i) s_bias[buf * kPairN + 32 * i + lane] = bias[i];
+        for (int i = 0; i < kWideN / 32; ++i) s_bias[buf * kWideN + 32 * i + lane] = bias[i];
         __syncwarp();
         if (lane == 0) mbar_arrive(bfull(buf));
         if (buf ^= 1u; buf == 0) bpar ^= 1u;
@@ -535,103 +647,107 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
     }
   } else {
     const int quad = warp & 3, half = warp >> 2;
-    const uint32_t src0 = tmem + (static_cast<uint32_t>(quad * 32) << 16) + half * kPairAccBufs * kPairCols;
-    const uint32_t dempty0 = map_to_cta(dempty(half, 0), 0);
-    const uint32_t out_smem = ring + kPairOutOff + warp * kOutWarp;
+    const uint32_t src0 = tmem + (static_cast<uint32_t>(quad * 32) << 16) + half * kWideCols;
+    const uint32_t out_smem = ring + kWideOutOff + warp * kOutBox;
     const uint32_t out_lane = out_smem + lane * 128 + ((lane & 7) << 4);   // piece i of the lane's row: at this address ^ 16 i
     const uint8_t *out_gen = smem_raw + (out_smem - smem_u32(smem_raw));
     uint32_t d = 0, dpar = 0, buf = 0, bpar = 0, s = 0, spar = 0;
     for (int it = first; it < n_items; it += stride) {
       const GemmTile t = tile_at(p, s_tiles, it, n_nb);
-      const int n0 = t.nb * kPairN + half * kPairCols;
-      uint64_t acc[kPairCols / 2];
+      const int n0 = t.nb * kWideN + half * kWideCols;
+      uint64_t acc[kWideCols / 2];
 #pragma unroll
-      for (int c = 0; c < kPairCols / 2; ++c) acc[c] = 0ull;
-      for (int kb = 0; kb < p.n_kb; ++kb) {
-        if (kb % kScaleBlocks == 0 && !mbar_wait_warp(sfull(s), spar, abort_flag, p.status, ST_WAIT_AREADY)) { ok = false; break; }
-        const float scale = s_scales[s * kPairScaleSlot + (half * kScaleBlocks + kb % kScaleBlocks) * 128 + quad * 32 + lane];
+      for (int c = 0; c < kWideCols / 2; ++c) acc[c] = 0ull;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if ((kb - kb0) % kScaleBlocks == 0 && !mbar_wait_warp(sfull(s), spar, abort_flag, p.status, ST_WAIT_AREADY)) { ok = false; break; }
+        const float scale = s_scales[s * kWideScaleSlot + (half * kScaleBlocks + (kb - kb0) % kScaleBlocks) * 128 + quad * 32 + lane];
         uint64_t f;
         asm("mov.b64 %0, {%1, %1};" : "=l"(f) : "r"(__float_as_uint(scale)));
-        if (!mbar_wait_warp<Wait::kClusterRelaxed>(dfull(half, d), dpar, abort_flag, p.status, ST_WAIT_DFULL)) { ok = false; break; }
+        if (!mbar_wait_warp(dfull(d), dpar, abort_flag, p.status, ST_WAIT_DFULL)) { ok = false; break; }
         tc_fence_after();
-        const uint32_t src = src0 + d * kPairCols;
+        const uint32_t src = src0 + d * kWideN;
         uint32_t v[2][16];
         tmem_ld16(src, v[0]);
 #pragma unroll
-        for (int c = 0; c < kPairCols / 16; ++c) {   // the next 16 columns are on their way while these are added
+        for (int c = 0; c < kWideCols / 16; ++c) {   // the next 16 columns are on their way while these are added
           tmem_wait_ld();
-          if (c + 1 < kPairCols / 16) {
+          if (c + 1 < kWideCols / 16) {
             tmem_ld16(src + 16 * (c + 1), v[(c + 1) & 1]);
           } else {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_relaxed_cluster(dempty0 + 8u * d);
+            if (lane == 0) mbar_arrive(dempty(d));
           }
 #pragma unroll
           for (int i = 0; i < 8; ++i) fma_f32x2(acc[8 * c + i], v[c & 1][2 * i], v[c & 1][2 * i + 1], f);
         }
-        if (kb % kScaleBlocks == kScaleBlocks - 1 || kb + 1 == p.n_kb) {
+        if ((kb - kb0) % kScaleBlocks == kScaleBlocks - 1 || kb + 1 == kb1) {
           __syncwarp();
           if (lane == 0) mbar_arrive(sempty(s));
-          if (++s == kPairScaleSlots) { s = 0; spar ^= 1u; }
+          if (++s == kScaleSlots) { s = 0; spar ^= 1u; }
         }
-        if (++d == kPairAccBufs) { d = 0; dpar ^= 1u; }
+        if (++d == kWideAccBufs) { d = 0; dpar ^= 1u; }
       }
       if (!ok) break;
-      // Through shared memory, boxes of 32 rows x 128 bytes: two of 64 16-bit columns, or twice two of 32 fp32 columns.  Rows
-      // that all exist leave by the copy engine while the next tile is under way, others (and outputs that it cannot
-      // address) by the warp, a row at a time.
-      const int rows_here = t.ntok - 128 * rank - quad * 32, row_out = t.row0 + 128 * rank + quad * 32;
+      if constexpr (kSplit) {   // every MMA of this CTA is complete: the ring takes the partial tile
+        float4 *part = reinterpret_cast<float4 *>(smem_raw + (ring - smem_u32(smem_raw))) + (quad * 32 + lane) * (kWidePart / 4) + half * (kWideCols / 4);
+#pragma unroll
+        for (int c = 0; c < kWideCols / 4; ++c)
+          part[c] = make_float4(__uint_as_float(static_cast<uint32_t>(acc[2 * c])), __uint_as_float(static_cast<uint32_t>(acc[2 * c] >> 32)),
+                                __uint_as_float(static_cast<uint32_t>(acc[2 * c + 1])), __uint_as_float(static_cast<uint32_t>(acc[2 * c + 1] >> 32)));
+        break;
+      }
+      // Through shared memory, a box of 32 rows x 128 bytes at a time: 64 16-bit columns or 32 fp32 ones.  Rows that all exist
+      // leave by the copy engine while the next box, or tile, is under way, others (and outputs that it cannot address) by the warp.
+      const int rows_here = t.ntok - quad * 32, row_out = t.row0 + quad * 32;
       const bool by_copy = tiled_out && rows_here >= 32;
-      auto leave = [&](int n, int box_cols) {   // both boxes, columns n..
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (by_copy) {
-          if (lane == 0) {
-            for (int i = 0; i < 2; ++i)
-              if (n + i * box_cols < p.n) tma_store_2d(&tm_out, n + i * box_cols, row_out, out_smem + i * kOutBox);
-            tma_store_commit();
-          }
-        } else {
-          copy_rows(p, out_gen, row_out, min(rows_here, 32), n, box_cols);
-        }
-      };
-      // (the address is formed inside the statement: sixteen of them, kept across the loop over k, would cost registers there)
-      auto stage = [&](int box, int piece, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
-        asm volatile("{\n\t.reg .b32 at;\n\txor.b32 at, %0, %1;\n\tadd.u32 at, at, %2;\n\tst.shared.v4.b32 [at], {%3, %4, %5, %6};\n\t}" ::"r"(out_lane),
-                     "r"(piece << 4), "r"(box * kOutBox), "r"(w0), "r"(w1), "r"(w2), "r"(w3)
-                     : "memory");
-      };
       if (!mbar_wait_warp(bfull(buf), bpar, abort_flag, p.status, ST_WAIT_AREADY)) { ok = false; break; }
-      const float4 *bias = reinterpret_cast<const float4 *>(s_bias + buf * kPairN + half * kPairCols);
+      const float4 *bias = reinterpret_cast<const float4 *>(s_bias + buf * kWideN + half * kWideCols);
       auto sums = [&](int c) {   // four columns with their bias
         const float4 b = bias[c];
         return make_float4(__uint_as_float(static_cast<uint32_t>(acc[2 * c])) + b.x, __uint_as_float(static_cast<uint32_t>(acc[2 * c] >> 32)) + b.y,
                            __uint_as_float(static_cast<uint32_t>(acc[2 * c + 1])) + b.z, __uint_as_float(static_cast<uint32_t>(acc[2 * c + 1] >> 32)) + b.w);
       };
-      if (lane == 0) tma_store_wait_read();   // of the tile before
-      __syncwarp();
+      // (the address is formed inside the statement: eight of them, kept across the loop over k, would cost registers there)
+      auto stage = [&](int piece, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
+        asm volatile("{\n\t.reg .b32 at;\n\txor.b32 at, %0, %1;\n\tst.shared.v4.b32 [at], {%2, %3, %4, %5};\n\t}" ::"r"(out_lane), "r"(piece << 4),
+                     "r"(w0), "r"(w1), "r"(w2), "r"(w3)
+                     : "memory");
+      };
+      auto box_free = [&]() {
+        if (lane == 0) tma_store_wait_read();
+        __syncwarp();
+      };
+      auto leave = [&](int n, int box_cols) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (by_copy) {
+          if (lane == 0 && n < p.n) {
+            tma_store_2d(&tm_out, n, row_out, out_smem);
+            tma_store_commit();
+          }
+        } else {
+          copy_box(p, out_gen, row_out, min(rows_here, 32), n);
+        }
+      };
       if (p.out_dtype == MOE_F32) {
 #pragma unroll
-        for (int c = 0; c < kPairCols / 4; ++c) {
-          if (c == kPairCols / 8) {
-            leave(n0, 32);
-            if (lane == 0) tma_store_wait_read();
-            __syncwarp();
-          }
+        for (int c = 0; c < kWideCols / 4; ++c) {
+          if (c % 8 == 0) box_free();
           const float4 v = sums(c);
-          stage(c / 8 % 2, c % 8, __float_as_uint(v.x), __float_as_uint(v.y), __float_as_uint(v.z), __float_as_uint(v.w));
+          stage(c % 8, __float_as_uint(v.x), __float_as_uint(v.y), __float_as_uint(v.z), __float_as_uint(v.w));
+          if (c % 8 == 7) leave(n0 + 4 * (c - 7), 32);
         }
-        leave(n0 + kPairCols / 2, 32);
       } else {
         const bool bf16 = p.out_dtype == MOE_BF16;
         auto pack = [&](float lo, float hi) { return bf16 ? pack2<__nv_bfloat16>(lo, hi) : pack2<__half>(lo, hi); };
 #pragma unroll
-        for (int c = 0; c < kPairCols / 8; ++c) {
+        for (int c = 0; c < kWideCols / 8; ++c) {
+          if (c % 8 == 0) box_free();
           const float4 v = sums(2 * c), u = sums(2 * c + 1);
-          stage(c / 8, c % 8, pack(v.x, v.y), pack(v.z, v.w), pack(u.x, u.y), pack(u.z, u.w));
+          stage(c % 8, pack(v.x, v.y), pack(v.z, v.w), pack(u.x, u.y), pack(u.z, u.w));
+          if (c % 8 == 7) leave(n0 + 8 * (c - 7), 64);
         }
-        leave(n0, 64);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(bempty(buf));
@@ -639,15 +755,33 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
     }
     if (lane == 0) tma_store_wait_all();
   }
+  __syncwarp();
+  if constexpr (kSplit) {
+    // the CTAs of the cluster add up the tile, each its share of the rows, in the order of k
+    cluster_sync_all();
+    if (first < n_items) {
+      const GemmTile t = tile_at(p, s_tiles, first, n_nb);
+      const int mine = (t.ntok - split + p.splits - 1) / p.splits;
+      for (int e = threadIdx.x; e < mine * (kWideN / 4); e += kWideThreads) {
+        const int row = split + e / (kWideN / 4) * p.splits, c = e % (kWideN / 4) * 4, n = t.nb * kWideN + c;
+        const float4 sum = sum_of_splits(ring + 4u * (row * kWidePart + c), p.splits);
+        const float o[4] = {sum.x, sum.y, sum.z, sum.w};
+        const size_t at = static_cast<size_t>(t.row0 + row) * p.ld_out + n;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (n + i < p.n) store_out(p, at + i, o[i] + (p.bias != nullptr ? __bfloat162float(p.bias[static_cast<size_t>(t.g) * p.n + n + i]) : 0.f));
+      }
+    }
+    cluster_sync_all();   // no CTA leaves while another may still read its part
+  }
   if (!ok && warp == kCopyWarp)   // give copies in flight time to land before shared memory is released
     for (int i = 0; i < 2000; ++i) __nanosleep(1000);
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  cluster_sync_all();   // neither CTA leaves while the pair's MMAs, copies or arrivals may still touch its memory
   if (warp == kMmaWarp) {
     tc_fence_after();
-    tmem_dealloc_pair(tmem, kPairAccBufs * kPairN);
+    tmem_dealloc(tmem, kWideAccBufs * kWideN);
   }
 }
 
@@ -683,37 +817,65 @@ struct GemmCall {
   Fp8GemmArgs p;
 };
 
+// CTAs that share the reduction of a tile where the call has at most `tiles`: as many as keep all of them resident, each with
+// some blocks of k, in a cluster of the size that every device takes.
+int k_splits(long long tiles, int n_kb, int sm_count) {
+  int splits = 1;
+  while (splits < kMaxSplits && tiles * splits * 2 <= sm_count && splits * 2 <= n_kb) splits *= 2;
+  return splits;
+}
+
+// Which kernel, by the rows that a group has (on average: their numbers are on the device).  us, the kernel with 16 / 64 / 128
+// token columns / the wide one; one product of 4096 x 7168: 1 row 8.3 / 9.0 / 10.0 / 12.5, 16 rows 8.7 / 9.3 / 9.8 / 13.2,
+// 64 rows 18 / 11.5 / 11.4 / 14.7, 128 rows 33 / 17.0 / 13.2 / 16.9, 256 rows 63 / 25.7 / 18.9 / 18.3; 32 groups of 5760 x 2880:
+// 8 rows each 90 / 85 / 89 / 96, 32 rows 162 / 93 / 94 / 100, 64 rows 293 / 137 / 104 / 102, 96 rows 423 / 191 / 113 / 104.
+// A tile narrower than its group reads the weights again, from L2; with a tail of groups above the average, columns for twice
+// the average pay.
+enum GemmForm { kForm16, kForm64, kForm128, kFormWide };
+GemmForm gemm_form(int rows, int n_groups, int n) {
+  const int per_group = (rows - 1) / n_groups + 1;
+  if (n_groups == 1 && per_group <= 16) return kForm16;
+  if (per_group <= (n_groups == 1 ? 64 : 32)) return kForm64;
+  if (per_group <= (n_groups == 1 ? 128 : 80) || n <= kScaleBlock) return kForm128;
+  return kFormWide;
+}
+
 template <int kTok>
-cudaError_t launch_fp8_gemm(const GemmCall &c, int sm_count, cudaStream_t s, bool &maps_ok) {
+cudaError_t launch_fp8_gemm(moe_ctx *h, const GemmCall &c, cudaStream_t s, bool &maps_ok) {
+  const int sm_count = h->sm_count;
   using S = GemmShape<kTok>;
   CUtensorMap ma, mb;
   maps_ok = encode_codes(&ma, c.a, c.k, c.ld_a, c.p.rows, 0, S::kBoxRows) && encode_codes(&mb, c.b, c.k, c.ld_b, c.p.n, c.p.n_groups, kScaleBlock);
   if (!maps_ok) return cudaSuccess;
-  cudaError_t e = cudaFuncSetAttribute(fp8_gemm_kernel<kTok>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+  const cudaError_t e = allow_smem(h, reinterpret_cast<const void *>(fp8_gemm_kernel<kTok>), S::kSmem, kTok == 16 ? kSmemGemm16 : kTok == 64 ? kSmemGemm64 : kSmemGemm128);
   if (e != cudaSuccess) return e;
   // Most tiles that the call can have: a group of cnt rows has at most 1 + (cnt - 1) / kTok.
   const long long groups = std::min(c.p.n_groups, c.p.rows), n_nb = (c.p.n + kScaleBlock - 1) / kScaleBlock;
   const long long most = (groups + (c.p.rows - groups) / kTok) * n_nb;
   Fp8GemmArgs p = c.p;
-  p.splits = 1;
-  while (p.splits < 8 && most * p.splits * 2 <= sm_count && p.splits * 2 <= p.n_kb) p.splits *= 2;
+  p.splits = k_splits(most, p.n_kb, sm_count);
+  const int wide = p.out_dtype != MOE_F32 && aligned_to(p.out, 16) && p.ld_out % 8 == 0;
   const dim3 grid(static_cast<unsigned>(p.splits > 1 ? most : std::min<long long>(most, sm_count)), p.splits, 1);
-  return launch_kernel(fp8_gemm_kernel<kTok>, grid, S::kThreads, S::kSmem, s, true, p.splits > 1 ? p.splits : 0, ma, mb, p);
+  return launch_kernel(fp8_gemm_kernel<kTok>, grid, S::kThreads, S::kSmem, s, true, p.splits > 1 ? p.splits : 0, ma, mb, p, wide);
 }
 
-cudaError_t launch_fp8_gemm_pair(const GemmCall &c, int sm_count, cudaStream_t s, bool &maps_ok) {
+cudaError_t launch_fp8_gemm_wide(moe_ctx *h, const GemmCall &c, cudaStream_t s, bool &maps_ok) {
+  const int sm_count = h->sm_count;
   CUtensorMap ma, mb;
-  maps_ok = encode_codes(&ma, c.a, c.k, c.ld_a, c.p.rows, 0, 128) && encode_codes(&mb, c.b, c.k, c.ld_b, c.p.n, c.p.n_groups, 64);
+  maps_ok = encode_codes(&ma, c.a, c.k, c.ld_a, c.p.rows, 0, 128) && encode_codes(&mb, c.b, c.k, c.ld_b, c.p.n, c.p.n_groups, kWideN);
   if (!maps_ok) return cudaSuccess;
-  const cudaError_t e = cudaFuncSetAttribute(fp8_gemm_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem);
+  const long long groups = std::min(c.p.n_groups, c.p.rows), n_nb = (c.p.n + kWideN - 1) / kWideN;
+  const long long most = (groups + (c.p.rows - groups) / kWideTok) * n_nb;
+  Fp8GemmArgs p = c.p;
+  p.splits = k_splits(most, p.n_kb, sm_count);
+  const auto kernel = p.splits > 1 ? fp8_gemm_wide_kernel<true> : fp8_gemm_wide_kernel<false>;
+  const cudaError_t e = allow_smem(h, reinterpret_cast<const void *>(kernel), kWideSmem, p.splits > 1 ? kSmemGemmWideSplit : kSmemGemmWide);
   if (e != cudaSuccess) return e;
-  const long long groups = std::min(c.p.n_groups, c.p.rows), n_nb = (c.p.n + kPairN - 1) / kPairN;
-  const long long most = (groups + (c.p.rows - groups) / kPairTok) * n_nb;
   // outputs through the copy engine: rows of 16-byte pieces
   CUtensorMap mo = ma;
   const int tiled = aligned_to(c.p.out, 16) && c.p.ld_out * dtype_size(c.p.out_dtype) % 16 == 0 && encode_out(&mo, c.p);
-  return launch_kernel(fp8_gemm_pair_kernel, dim3(2 * static_cast<unsigned>(std::min<long long>(most, sm_count / 2)), 1, 1), kPairThreads, kPairSmem, s,
-                       true, 0, ma, mb, mo, c.p, tiled);
+  const dim3 grid(static_cast<unsigned>(p.splits > 1 ? most : std::min<long long>(most, sm_count)), p.splits, 1);
+  return launch_kernel(kernel, grid, kWideThreads, kWideSmem, s, true, p.splits > 1 ? p.splits : 0, ma, mb, mo, p, tiled);
 }
 
 }  // namespace
@@ -748,13 +910,12 @@ int moe_gemm_fp8(moe_handle c, const uint8_t *a_dev, long long ld_a, const float
   p.bias = static_cast<const __nv_bfloat16 *>(bias_dev); p.out = out_dev; p.ld_out = static_cast<size_t>(ld_out);
   p.out_dtype = out_dtype; p.status = c->status;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int per_group = (rows - 1) / n_groups + 1;
+  const GemmForm form = gemm_form(rows, n_groups, n);
   bool maps_ok = true;
-  const cudaError_t e = per_group > 96 && n > kScaleBlock ? launch_fp8_gemm_pair(call, c->sm_count, s, maps_ok)
-                        : per_group <= 16   ? launch_fp8_gemm<16>(call, c->sm_count, s, maps_ok)
-                        : per_group <= 32 ? launch_fp8_gemm<32>(call, c->sm_count, s, maps_ok)
-                        : per_group <= 64 ? launch_fp8_gemm<64>(call, c->sm_count, s, maps_ok)
-                                          : launch_fp8_gemm<128>(call, c->sm_count, s, maps_ok);
+  const cudaError_t e = form == kForm16    ? launch_fp8_gemm<16>(c, call, s, maps_ok)
+                        : form == kForm64  ? launch_fp8_gemm<64>(c, call, s, maps_ok)
+                        : form == kForm128 ? launch_fp8_gemm<128>(c, call, s, maps_ok)
+                                           : launch_fp8_gemm_wide(c, call, s, maps_ok);
   if (!maps_ok) return op_fail(c, MOE_ERR_INVALID, "moe_gemm_fp8: no tensor map for %d x %d and %d x %d x %d codes", rows, k, n_groups, n, k);
   return launched(c, "moe_gemm_fp8", e);
 }

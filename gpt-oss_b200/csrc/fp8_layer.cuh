@@ -29,6 +29,14 @@ inline int use_device(moe_ctx *c, const char *who) {
   const cudaError_t e = cudaSetDevice(c->cfg.device);
   return e == cudaSuccess ? MOE_OK : op_fail(c, MOE_ERR_CUDA, "%s: cudaSetDevice(%d): %s", who, c->cfg.device, cudaGetErrorString(e));
 }
+// Dynamic shared memory above 48 KB has to be asked for, once per kernel and device: bits of moe_ctx::smem_asked.
+enum : unsigned { kSmemGemm16 = 1u, kSmemGemm64 = 2u, kSmemGemm128 = 4u, kSmemGemmWide = 8u, kSmemGemmWideSplit = 16u, kSmemGroup = 32u };
+inline cudaError_t allow_smem(moe_ctx *c, const void *kernel, int bytes, unsigned bit) {
+  if (c->smem_asked & bit) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) c->smem_asked |= bit;
+  return e;
+}
 inline int launched(moe_ctx *c, const char *who, cudaError_t e) {
   if (e != cudaSuccess) {
     (void)cudaGetLastError();   // a refused launch is not left for the next call to find

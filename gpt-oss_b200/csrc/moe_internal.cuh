@@ -73,12 +73,12 @@ __host__ __device__ inline size_t w_scales_offset(int kc, int n_kc) {
 
 // Device status bits (MOE_DBG_STATUS).
 enum : unsigned {
-  ST_WAIT_FULL = 1u,      // expert GEMM: TMA data never arrived
-  ST_WAIT_EMPTY = 2u,     // expert GEMM: stage never released
-  ST_WAIT_AREADY = 4u,    // expert GEMM: dequantised tile never published
-  ST_WAIT_AFREE = 8u,     // expert GEMM: tensor-memory A buffer never released
-  ST_WAIT_DFULL = 16u,    // expert GEMM: accumulator never completed
-  ST_WAIT_DEMPTY = 32u,   // expert GEMM: accumulator never drained
+  ST_WAIT_FULL = 1u,      // a GEMM: TMA data never arrived
+  ST_WAIT_EMPTY = 2u,     // a GEMM: stage never released
+  ST_WAIT_AREADY = 4u,    // expert GEMM: SwiGLU rows of a tile never counted; FP8 GEMM: scales or bias never handed over
+  ST_WAIT_AFREE = 8u,     // FP8 GEMM: slot of scales or bias never released
+  ST_WAIT_DFULL = 16u,    // a GEMM: accumulator never completed
+  ST_WAIT_DEMPTY = 32u,   // a GEMM: accumulator never drained
   ST_BAD_INDEX = 64u,     // routing produced an out-of-range row
   ST_WAIT_PEER = 128u,    // TP collective: a peer's flag never arrived
   ST_Y_RANGE = 256u,      // expert GEMM: an MLP2 output does not fit fp16 (|y| > 65504)
@@ -235,6 +235,7 @@ struct moe_ctx {
   int *n_work = nullptr;            // [2]
   int max_work1 = 0, max_work2 = 0;
   unsigned int *status = nullptr;
+  unsigned smem_asked = 0;          // kernels whose shared memory was asked for (fp8_layer.cuh)
   int last_rows = 0;
   long long launches = 0;
   moe::TpPeers peers = {};          // TP group view; own entries are set at creation

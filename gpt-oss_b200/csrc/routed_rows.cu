@@ -287,7 +287,7 @@ int moe_group_pairs(moe_handle c, const int *idx_dev, int rows, int top_k, int n
     return op_fail(c, MOE_ERR_INVALID, "moe_group_pairs: a tensor is not aligned to its elements");
   if (int rc = use_device(c, "moe_group_pairs")) return rc;
   const size_t smem = static_cast<size_t>(kGroupWarps) * n_experts * sizeof(int);
-  cudaError_t e = cudaFuncSetAttribute(group_pairs_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGroupWarps * kMaxGroupedExperts * 4);
+  cudaError_t e = allow_smem(c, reinterpret_cast<const void *>(group_pairs_kernel), kGroupWarps * kMaxGroupedExperts * 4, kSmemGroup);
   if (e == cudaSuccess) {
     group_pairs_kernel<<<1, kGroupThreads, smem, static_cast<cudaStream_t>(stream)>>>(idx_dev, static_cast<size_t>(rows) * top_k, n_experts,
                                                                                       offsets_dev, pair_row_dev, row_pair_dev);
