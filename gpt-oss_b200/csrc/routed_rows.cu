@@ -3,6 +3,7 @@
 // (moe_combine_pairs).  The MXFP4 block has fixed forms of all three inside (route.cu); these take any router rule, any
 // row types and strides, and pairs without an expert.
 #include "fp8_layer.cuh"
+#include "sm100_ptx.cuh"
 
 namespace moe {
 
@@ -10,119 +11,264 @@ namespace moe {
 // Routing.  Of a row's logits x:  s = sigmoid(x), or softmax over the experts that are on;  p = s + bias;  the groups
 // with the highest sum of their group_top largest p stay;  the top_k largest p of what stays are selected, ties to the
 // lower index;  weight = s [/ sum of the selected s] * scale.  An expert is off where x or its bias is -inf or NaN.
-// Scores are held in 64 bits: which of two neighbouring p is larger is part of the answer, and s + bias is where
-// 32 bits would tie or swap them.
+//
+// Which of two neighbouring p is larger is part of the answer, so the comparisons are those of 64 bits.  A row is tried in
+// 32 bits first: there an s is off by less than 2^-18 of the row's largest possible s (exp, a sum of up to 512, a quotient), so
+// an order is certain where the two values differ by 2^-17 of it and 2^-22 of their own magnitudes (twice that for sums of two).
+// A row with a closer call (equal scores, scores that saturate) is done again in 64 bits.
+//
 // A warp per row; lane l owns the per_lane consecutive experts from l * per_lane, so that a lower lane is a lower index.
 // ---------------------------------------------------------------------------
 constexpr int kRouteWarps = 4;
 constexpr int kMaxScoredExperts = 512, kMaxScoredTopK = 32, kMaxScoredGroups = 32;
 
-// 64-bit integers in the order of the doubles; 0 is below every one of them and means "off".
-__device__ __forceinline__ unsigned long long ordered_key(double p) {
-  const long long b = __double_as_longlong(p == 0.0 ? 0.0 : p);   // -0 and 0 are equal
-  return b < 0 ? ~static_cast<unsigned long long>(b) : static_cast<unsigned long long>(b) | 0x8000000000000000ull;
+// Unsigned integers in the order of the values; 0 is below every one of them and means "off".
+__device__ __forceinline__ unsigned ordered_key(float p) {
+  const unsigned b = __float_as_uint(p + 0.f);   // -0 and 0 are equal
+  return (b >> 31) ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ unsigned long long ordered_key(double p) {
+  const unsigned long long b = static_cast<unsigned long long>(__double_as_longlong(p + 0.0));
+  return (b >> 63) ? ~b : b | 0x8000000000000000ull;
+}
+__device__ __forceinline__ float key_value(unsigned k) { return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k); }
 __device__ __forceinline__ double key_value(unsigned long long k) {
   return __longlong_as_double(static_cast<long long>((k >> 63) ? k & 0x7fffffffffffffffull : ~k));
+}
+// Largest key of the warp and the lanes that have it.
+__device__ __forceinline__ unsigned warp_best(unsigned k, unsigned &owners) {
+  const unsigned top = __reduce_max_sync(0xffffffffu, k);
+  owners = __ballot_sync(0xffffffffu, k == top);
+  return top;
+}
+__device__ __forceinline__ unsigned long long warp_best(unsigned long long k, unsigned &owners) {
+  const unsigned hi = static_cast<unsigned>(k >> 32), lo = static_cast<unsigned>(k);
+  const unsigned hi_top = __reduce_max_sync(0xffffffffu, hi);
+  const unsigned lo_top = __reduce_max_sync(0xffffffffu, hi == hi_top ? lo : 0u);
+  owners = __ballot_sync(0xffffffffu, hi == hi_top && lo == lo_top);
+  return static_cast<unsigned long long>(hi_top) << 32 | lo_top;
+}
+template <class R>
+__device__ __forceinline__ R warp_sum(R v) {
+#pragma unroll
+  for (int off = 16; off; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  return v;
+}
+
+// One row with scores of type R.  x[i]: the lane's logits, -inf where there is none.  Lane k < top_k receives the k-th selected
+// expert (or -1) in `sel`.  R = float: returns false where 32 bits do not settle a comparison.  `top` and `sum`: of the softmax.
+// `group_lanes`: lanes of a group, where groups are runs of whole lanes, a power of two of them; else 0 and `shared` is used.
+template <class R, int kPer>
+__device__ __forceinline__ bool select_experts(const float (&x)[kPer], const float *bias, const moe_route_rule &rule, int per_lane, int group_lanes,
+                                               unsigned long long *shared, int lane, float top, double &sum, int &sel, R &sel_s) {
+  constexpr bool kFast = sizeof(R) == 4;
+  using Key = decltype(ordered_key(R()));
+  const float inf = __int_as_float(0x7f800000);
+  const int first = lane * per_lane;
+  R s[kPer];
+  Key key[kPer];
+  R bound = 1;   // no s is larger
+  if (rule.score == MOE_SCORE_SOFTMAX) {
+    R part = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if constexpr (kFast) s[i] = x[i] > -inf ? __expf(x[i] - top) : 0.f;
+      else s[i] = x[i] > -inf ? exp(static_cast<double>(x[i]) - static_cast<double>(top)) : 0.0;
+      part += s[i];
+    }
+    part = warp_sum(part);
+    sum = part;
+    bound = part > 0 ? R(1) / part : R(0);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if constexpr (kFast) s[i] *= bound;
+      else if (part > 0) s[i] /= part;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if constexpr (kFast) s[i] = __fdividef(1.f, 1.f + __expf(-x[i]));
+      else s[i] = 1.0 / (1.0 + exp(-static_cast<double>(x[i])));
+    }
+  }
+  const R close = bound * R(7.62939453125e-06), rel = R(2.384185791015625e-07);   // 2^-17, 2^-22
+  auto certain = [&](Key a, Key b, R twice) {   // a is the larger of two keys that are on
+    const R va = key_value(a), vb = key_value(b);
+    return va - vb > twice * (close + rel * (fabs(va) + fabs(vb)));
+  };
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    key[i] = 0;
+    if (i < per_lane && x[i] > -inf) {
+      const float b = bias != nullptr ? bias[first + i] : 0.f;
+      if (b > -inf) key[i] = ordered_key(s[i] + static_cast<R>(b));
+    }
+  }
+  bool settled = true;
+  if (rule.n_groups > 1) {
+    // lane g < n_groups: what group g is worth, from its two largest
+    const int size = rule.n_experts / rule.n_groups;
+    Key k1 = 0, k2 = 0;
+    if (kFast || group_lanes > 0) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        k2 = max(k2, min(k1, key[i]));
+        k1 = max(k1, key[i]);
+      }
+      for (int off = 1; off < group_lanes; off <<= 1) {
+        const Key o1 = __shfl_xor_sync(0xffffffffu, k1, off), o2 = __shfl_xor_sync(0xffffffffu, k2, off);
+        k2 = max(max(k2, o2), min(k1, o1));
+        k1 = max(k1, o1);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (i < per_lane && first + i < rule.n_experts) shared[first + i] = key[i];
+      __syncwarp();
+      if (lane < rule.n_groups)
+        for (int j = 0; j < size; ++j) {
+          const Key k = static_cast<Key>(shared[lane * size + j]);
+          k2 = max(k2, min(k1, k));
+          k1 = max(k1, k);
+        }
+    }
+    Key worth = k1;
+    if (rule.group_top == 2 && k2) worth = ordered_key(key_value(k1) + key_value(k2));
+    if (group_lanes > 0) worth = __shfl_sync(0xffffffffu, worth, lane * group_lanes & 31);
+    if (lane >= rule.n_groups) worth = 0;
+    int better = 0;
+    for (int g = 0; g < rule.n_groups; ++g) {
+      const Key k = __shfl_sync(0xffffffffu, worth, g);
+      better += k > worth || (k == worth && g < lane);
+    }
+    const unsigned stays = __ballot_sync(0xffffffffu, lane < rule.n_groups && better < rule.top_groups);
+    if (kFast && rule.top_groups < rule.n_groups) {   // the last group that stays against the first that does not
+      const unsigned in = __ballot_sync(0xffffffffu, lane < rule.n_groups && better == rule.top_groups - 1);
+      const unsigned out = __ballot_sync(0xffffffffu, lane < rule.n_groups && better == rule.top_groups);
+      const Key a = __shfl_sync(0xffffffffu, worth, __ffs(in) - 1), b = __shfl_sync(0xffffffffu, worth, __ffs(out) - 1);
+      if (b != 0 && !certain(a, b, R(2))) settled = false;
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (i < per_lane && first + i < rule.n_experts && !(stays >> ((first + i) / size) & 1u)) key[i] = 0;
+  }
+  // rounds: the largest key of a lane, then of the warp; the lowest lane of equal ones.  In 32 bits one round more, for the
+  // first that is not selected.
+  sel = -1;
+  sel_s = 0;
+  Key best = 0, last = 0;
+  int at = 0;
+  auto find = [&]() {
+    best = key[0];
+    at = 0;
+#pragma unroll
+    for (int i = 1; i < kPer; ++i)
+      if (key[i] > best) { best = key[i]; at = i; }
+  };
+  find();
+  for (int k = 0; k < rule.top_k + (kFast ? 1 : 0); ++k) {
+    unsigned owners;
+    const Key top_key = warp_best(best, owners);
+    if (top_key == 0) break;   // nothing left
+    if (kFast && k > 0 && !certain(last, top_key, R(1))) settled = false;
+    if (kFast && (__popc(owners) > 1 || !settled)) { settled = false; break; }
+    last = top_key;
+    const int owner = __ffs(owners) - 1, e = __shfl_sync(0xffffffffu, first + at, owner);
+    if (lane == k && k < rule.top_k) sel = e;
+    if (!kFast) {
+      R es = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (i == at) es = s[i];
+      es = __shfl_sync(0xffffffffu, es, owner);
+      if (lane == k) sel_s = es;
+    }
+    if (lane == owner) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (i == at) key[i] = 0;
+      find();
+    }
+  }
+  return settled;
 }
 
 template <class T, int kPer>
 __global__ void __launch_bounds__(kRouteWarps * 32)
-route_scored_kernel(const T *logits, size_t ld, const float *bias, int rows, moe_route_rule rule, int per_lane, int *idx, float *w) {
-  __shared__ unsigned long long s_keys[kRouteWarps][kPer * 32];
+route_scored_kernel(const T *logits, size_t ld, const float *bias, int rows, moe_route_rule rule, int per_lane, int group_lanes, int vec, int *idx,
+                    float *w) {
+  __shared__ unsigned long long s_keys[kRouteWarps][kPer * 32];   // groups that are not whole lanes
+  grid_dep_sync();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const size_t row = static_cast<size_t>(blockIdx.x) * kRouteWarps + warp;
   if (row >= static_cast<size_t>(rows)) return;
   const int E = rule.n_experts, first = lane * per_lane;
   const float inf = __int_as_float(0x7f800000);
-  double s[kPer];
-  unsigned long long key[kPer];
-  double top = -1e300;   // largest logit of the experts that are on
+  float x[kPer];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const bool mine = i < per_lane && first + i < E;
-    float x = mine ? to_f32(logits[row * ld + first + i]) : -inf;
-    if (x > 3.402823466e38f) x = 3.402823466e38f;   // +inf counts as the largest finite value
-    key[i] = x > -inf ? 1 : 0;
-    s[i] = x;
-    if (key[i]) top = fmax(top, s[i]);
-  }
-  if (rule.score == MOE_SCORE_SOFTMAX) {
-    for (int off = 16; off; off >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, off));
-    double sum = 0.0;
+  for (int i = 0; i < kPer; ++i) x[i] = -inf;
+  const T *src = logits + row * ld;
+  constexpr int kVec = 16 / static_cast<int>(sizeof(T));
+  if (kPer >= kVec && vec) {   // per_lane is a multiple of kVec, rows are 16-byte aligned
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      s[i] = key[i] ? exp(s[i] - top) : 0.0;
-      sum += s[i];
-    }
-    for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    for (int i = 0; i + kVec <= kPer; i += kVec)
+      if (i < per_lane && first + i < E) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(src + first + i);
+        const T *e = reinterpret_cast<const T *>(&v);
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (key[i]) s[i] /= sum;
+        for (int j = 0; j < kVec; ++j) x[i + j] = to_f32(e[j]);
+      }
   } else {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) s[i] = key[i] ? 1.0 / (1.0 + exp(-s[i])) : 0.0;
+    for (int i = 0; i < kPer; ++i)
+      if (i < per_lane && first + i < E) x[i] = to_f32(src[first + i]);
   }
+  float top = -inf;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    if (!key[i]) continue;
-    const float b = bias != nullptr ? bias[first + i] : 0.f;
-    key[i] = b > -inf ? ordered_key(s[i] + static_cast<double>(b)) : 0;
+    if (x[i] > 3.402823466e38f) x[i] = 3.402823466e38f;   // +inf counts as the largest finite value
+    if (x[i] != x[i]) x[i] = -inf;                         // NaN is off
+    top = fmaxf(top, x[i]);
   }
-  if (rule.n_groups > 1) {
-    // lane g takes group g: the group_top largest of its members, then its rank among the groups
+  if (rule.score == MOE_SCORE_SOFTMAX) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (i < per_lane && first + i < E) s_keys[warp][first + i] = key[i];
-    __syncwarp();
-    const int size = E / rule.n_groups;
-    unsigned long long k1 = 0, k2 = 0;
-    if (lane < rule.n_groups)
-      for (int j = 0; j < size; ++j) {
-        const unsigned long long k = s_keys[warp][lane * size + j];
-        if (k > k1) { k2 = k1; k1 = k; }
-        else if (k > k2) k2 = k;
+    for (int off = 16; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    if (!(top > -inf)) top = 0.f;
+  }
+  int sel;
+  double sum = 0.0, share = 0.0;
+  float unused;
+  if ((rule.n_groups == 1 || group_lanes > 0) &&
+      select_experts<float, kPer>(x, bias, rule, per_lane, group_lanes, nullptr, lane, top, sum, sel, unused)) {
+    // weights of the selected from their logits, within a few roundings of 32 bits
+    float s = 0.f;
+    if (sel >= 0) {
+      float v = to_f32(src[sel]);
+      if (v > 3.402823466e38f) v = 3.402823466e38f;
+      if (rule.score == MOE_SCORE_SOFTMAX) {
+        const float d = v - top, r = d - v, lost = (v - (d - r)) - (top + r);   // v - top is d + lost exactly
+        s = expf(d);
+        if (fabsf(lost) < 1.f) s = fmaf(s, lost, s);
+      } else {
+        s = __fdiv_rn(1.f, 1.f + expf(-v));
       }
-    unsigned long long g_key = k1;
-    if (rule.group_top == 2 && k2) g_key = ordered_key(key_value(k1) + key_value(k2));
-    int better = 0;
-    for (int g = 0; g < rule.n_groups; ++g) {
-      const unsigned long long k = __shfl_sync(0xffffffffu, g_key, g);
-      better += k > g_key || (k == g_key && g < lane);
     }
-    const unsigned stays = __ballot_sync(0xffffffffu, lane < rule.n_groups && better < rule.top_groups);
-#pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (i < per_lane && first + i < E && !(stays >> ((first + i) / size) & 1u)) key[i] = 0;
-  }
-  // top_k rounds: the largest key of a lane, then of the warp; the lowest lane of equal ones
-  int sel = -1;
-  double sel_s = 0.0;
-  for (int k = 0; k < rule.top_k; ++k) {
-    unsigned long long best = 0;
-    int at = 0;
-    double best_s = 0.0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (key[i] > best) { best = key[i]; at = i; best_s = s[i]; }
-    const unsigned hi = static_cast<unsigned>(best >> 32), lo = static_cast<unsigned>(best);
-    const unsigned hi_max = __reduce_max_sync(0xffffffffu, hi);
-    if (hi_max == 0) break;   // nothing left (a key that is on has its sign bit or a large complement set)
-    const unsigned lo_max = __reduce_max_sync(0xffffffffu, hi == hi_max ? lo : 0u);
-    const int owner = __ffs(__ballot_sync(0xffffffffu, hi == hi_max && lo == lo_max)) - 1;
-    const int e = __shfl_sync(0xffffffffu, first + at, owner);
-    const double es = __shfl_sync(0xffffffffu, best_s, owner);
-    if (lane == k) { sel = e; sel_s = es; }
-    if (lane == owner) {
-#pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (i == at) key[i] = 0;
+    if (rule.renormalise) {
+      const float all = warp_sum(s);
+      share = all > 0.f ? __fdiv_rn(s, all) : 0.f;
+    } else {
+      share = rule.score == MOE_SCORE_SOFTMAX && sum > 0.0 ? s / sum : s;
+    }
+  } else {
+    double s;
+    select_experts<double, kPer>(x, bias, rule, per_lane, group_lanes, s_keys[warp], lane, top, sum, sel, s);
+    share = s;
+    if (rule.renormalise) {
+      const double all = warp_sum(s);
+      share = all > 0.0 ? s / all : 0.0;
     }
   }
-  double sum = sel_s;
-  for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
   if (lane < rule.top_k) {
-    const double share = !rule.renormalise ? sel_s : sum > 0.0 ? sel_s / sum : 0.0;
     idx[row * rule.top_k + lane] = sel;
     w[row * rule.top_k + lane] = static_cast<float>(share * static_cast<double>(rule.scale));
   }
@@ -131,50 +277,90 @@ route_scored_kernel(const T *logits, size_t ld, const float *bias, int rows, moe
 template <class T>
 cudaError_t launch_route_scored(const moe_route_rule &r, const void *logits, size_t ld, const float *bias, int rows, int *idx, float *w,
                                 cudaStream_t s) {
-  const int per = (r.n_experts + 31) / 32;
+  // Experts of a lane: enough for all in 32 lanes; with groups, up to 16 such that a group is a power of two of whole lanes.
+  int per = (r.n_experts + 31) / 32, group_lanes = 0;
+  if (r.n_groups > 1) {
+    const int size = r.n_experts / r.n_groups;
+    for (int p = per; p <= 16 && group_lanes == 0; ++p)
+      if (size % p == 0 && ((size / p) & (size / p - 1)) == 0) { per = p; group_lanes = size / p; }
+  }
   const unsigned grid = static_cast<unsigned>((static_cast<size_t>(rows) + kRouteWarps - 1) / kRouteWarps);
   const T *x = static_cast<const T *>(logits);
-  auto go = [&](auto kernel) { kernel<<<grid, kRouteWarps * 32, 0, s>>>(x, ld, bias, rows, r, per, idx, w); };
-  if (per <= 1) go(route_scored_kernel<T, 1>);
-  else if (per <= 2) go(route_scored_kernel<T, 2>);
-  else if (per <= 4) go(route_scored_kernel<T, 4>);
-  else if (per <= 8) go(route_scored_kernel<T, 8>);
-  else go(route_scored_kernel<T, 16>);
-  return cudaGetLastError();
+  constexpr int kVec = 16 / static_cast<int>(sizeof(T));
+  const int vec = per % kVec == 0 && r.n_experts % kVec == 0 && ld % kVec == 0 && aligned_to(x, 16);
+  auto go = [&](auto kernel) {
+    return launch_kernel(kernel, dim3(grid), kRouteWarps * 32, 0, s, true, 0, x, ld, bias, rows, r, per, group_lanes, vec, idx, w);
+  };
+  if (per <= 1) return go(route_scored_kernel<T, 1>);
+  if (per <= 2) return go(route_scored_kernel<T, 2>);
+  if (per <= 4) return go(route_scored_kernel<T, 4>);
+  if (per <= 8) return go(route_scored_kernel<T, 8>);
+  return go(route_scored_kernel<T, 16>);
 }
 
 // ---------------------------------------------------------------------------
-// Stable counting sort of the pairs (token * top_k + slot) by expert.  One CTA: every warp owns a contiguous range of
-// pairs and counts it into a histogram of its own; prefixes over experts and warps give every warp its place in every
-// expert's rows; a second walk over the same pairs hands the places out, so that they ascend with the pair.
+// Stable counting sort of the pairs (token * top_k + slot) by expert, in one launch of one cluster: the CTAs own contiguous
+// ranges of pairs and their warps contiguous parts of them, each with a histogram of its own.  Every CTA reads the others'
+// totals from their shared memory; prefixes over experts, CTAs and warps then give every warp its place in every expert's rows,
+// and a second walk over the same pairs hands the places out, so that they ascend with the pair.  Latency is all there is to
+// it: 8192 x 8 pairs 80 us on one CTA, of which 16 walks of a warp over 64 pairs each are left on eight.
 // ---------------------------------------------------------------------------
-constexpr int kGroupThreads = 1024, kGroupWarps = kGroupThreads / 32;
+constexpr int kGroupThreads = 1024, kGroupWarps = kGroupThreads / 32, kGroupMaxCtas = 8;
 constexpr int kMaxGroupedExperts = 1024;
 
 __global__ void __launch_bounds__(kGroupThreads)
 group_pairs_kernel(const int *idx, size_t n_pairs, int E, int *offsets, int *pair_row, int *row_pair) {
-  extern __shared__ int s_hist[];   // [kGroupWarps][E]
-  __shared__ int s_scan[kGroupWarps], s_total;
+  extern __shared__ int s_hist[];   // [kGroupWarps][E], then the totals of this CTA [E]
+  __shared__ int s_scan[kGroupWarps], s_all;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int *mine = s_hist + warp * E;
+  const int ctas = gridDim.y, rank = blockIdx.y;   // the cluster is the grid
+  int *mine = s_hist + warp * E, *totals = s_hist + kGroupWarps * E;
   for (int i = threadIdx.x; i < kGroupWarps * E; i += kGroupThreads) s_hist[i] = 0;
   __syncthreads();
-  const size_t per = (n_pairs + kGroupThreads - 1) / kGroupThreads * 32;
-  const size_t begin = min(per * warp, n_pairs), end = min(begin + per, n_pairs);
-  for (size_t p = begin + lane; p < end; p += 32) {
+  grid_dep_sync();
+  const size_t per = (n_pairs + static_cast<size_t>(ctas) * kGroupThreads - 1) / (static_cast<size_t>(ctas) * kGroupThreads) * 32;
+  const size_t begin = min(per * (rank * kGroupWarps + warp), n_pairs), end = min(begin + per, n_pairs);
+  // the first eight steps of a warp stay in registers for the second walk
+  constexpr int kKept = 8;
+  int kept[kKept];
+#pragma unroll
+  for (int i = 0; i < kKept; ++i) {
+    const size_t p = begin + 32 * i + lane;
+    kept[i] = p < end ? idx[p] : -1;
+    if (kept[i] >= E) kept[i] = -1;
+  }
+#pragma unroll
+  for (int i = 0; i < kKept; ++i)
+    if (kept[i] >= 0) atomicAdd(&mine[kept[i]], 1);
+  for (size_t p = begin + 32 * kKept + lane; p < end; p += 32) {
     const int e = idx[p];
     if (e >= 0 && e < E) atomicAdd(&mine[e], 1);
   }
   __syncthreads();
-  // thread e: exclusive prefix over the warps, then over the experts
+  // thread e: exclusive prefix over the warps of this CTA, then over the CTAs and the experts
   int total = 0;
-  if (threadIdx.x < E)
+  if (threadIdx.x < E) {
     for (int v = 0; v < kGroupWarps; ++v) {
       const int n = s_hist[v * E + threadIdx.x];
       s_hist[v * E + threadIdx.x] = total;
       total += n;
     }
-  int incl = total;
+    totals[threadIdx.x] = total;
+  }
+  int before = 0, all = total;
+  if (ctas > 1) {
+    sm100::cluster_sync_all();
+    all = 0;
+    if (threadIdx.x < E)
+#pragma unroll
+      for (int r = 0; r < kGroupMaxCtas; ++r)
+        if (r < ctas) {
+          const int n = static_cast<int>(sm100::ld_cluster_u32(sm100::map_to_cta(sm100::smem_u32(&totals[threadIdx.x]), r)));
+          all += n;
+          if (r < rank) before += n;
+        }
+  }
+  int incl = all;
   for (int off = 1; off < 32; off <<= 1) {
     const int up = __shfl_up_sync(0xffffffffu, incl, off);
     if (lane >= off) incl += up;
@@ -188,60 +374,155 @@ group_pairs_kernel(const int *idx, size_t n_pairs, int E, int *offsets, int *pai
       if (lane >= off) t += up;
     }
     s_scan[lane] = t - v;
-    if (lane == 31) s_total = t;
+    if (lane == 31) s_all = t;
   }
   __syncthreads();
-  const int start = s_scan[warp] + incl - total;
+  const int start = s_scan[warp] + incl - all;
   if (threadIdx.x < E) {
-    offsets[threadIdx.x] = start;
-    for (int v = 0; v < kGroupWarps; ++v) s_hist[v * E + threadIdx.x] += start;
+    if (rank == 0) offsets[threadIdx.x] = start;
+    for (int v = 0; v < kGroupWarps; ++v) s_hist[v * E + threadIdx.x] += start + before;
   }
-  if (threadIdx.x == 0) offsets[E] = s_total;
+  if (rank == 0 && threadIdx.x == 0) offsets[E] = s_all;
   __syncthreads();
-  for (size_t p0 = begin; p0 < end; p0 += 32) {
-    const size_t p = p0 + lane;
-    int e = p < end ? idx[p] : -1;
-    if (e < 0 || e >= E) e = -1;
+  auto place = [&](size_t p, int e) {
     const unsigned same = __match_any_sync(0xffffffffu, e);
-    const int rank = __popc(same & ((1u << lane) - 1u));
+    const int rank_here = __popc(same & ((1u << lane) - 1u));
     int row = -1;
-    if (e >= 0) row = mine[e] + rank;
+    if (e >= 0) row = mine[e] + rank_here;
     __syncwarp();
-    if (e >= 0 && rank == 0) mine[e] += __popc(same);
+    if (e >= 0 && rank_here == 0) mine[e] += __popc(same);
     __syncwarp();
     if (p < end) pair_row[p] = row;
     if (row >= 0 && row_pair != nullptr) row_pair[row] = static_cast<int>(p);
+  };
+#pragma unroll
+  for (int i = 0; i < kKept; ++i)
+    if (begin + 32 * i < end) place(begin + 32 * i + lane, kept[i]);
+  for (size_t p0 = begin + 32 * kKept; p0 < end; p0 += 32) {
+    const size_t p = p0 + lane;
+    int e = p < end ? idx[p] : -1;
+    if (e < 0 || e >= E) e = -1;
+    place(p, e);
   }
   if (row_pair != nullptr)
-    for (size_t r = static_cast<size_t>(s_total) + threadIdx.x; r < n_pairs; r += kGroupThreads) row_pair[r] = -1;
+    for (size_t r = static_cast<size_t>(s_all) + rank * kGroupThreads + threadIdx.x; r < n_pairs; r += static_cast<size_t>(ctas) * kGroupThreads)
+      row_pair[r] = -1;
+  if (ctas > 1) sm100::cluster_sync_all();   // no CTA leaves while another may still read its totals
 }
 
 // ---------------------------------------------------------------------------
 // out[t] = residual[t] + sum over k of w[t, k] * y[pair_row[t, k]], added in the order of k in fp32 and rounded once.
 // A pair whose row is negative or not below n_y_rows adds nothing, whatever its weight.
 // ---------------------------------------------------------------------------
+// Bound by HBM.  A CTA per row (per part of one where there are few rows); a thread has eight neighbouring columns a step.  With
+// every row 16-byte aligned (vec) they are one or two wide loads, and the loads of four pairs are requested together and a step
+// ahead of their use.  8192 rows of 2880 bf16 columns, four pairs each, us: a CTA per 1024 columns 61 (the loads of an index and
+// of the row behind it are then most of a CTA's life), per row, a step ahead 40.
+constexpr int kCombineThreads = 128, kCombineCols = 8;
+
+template <class T>
+struct Raw8 {   // eight values as they lie in memory
+  uint4 v[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T *p) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) v[i] = reinterpret_cast<const uint4 *>(p)[i];
+  }
+  __device__ __forceinline__ float operator[](int i) const { return to_f32(reinterpret_cast<const T *>(v)[i]); }
+};
+template <class T>
+__device__ __forceinline__ void store8(T *p, const float (&v)[8]) {
+  uint4 raw[sizeof(T) / 2];
+  T *e = reinterpret_cast<T *>(raw);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) store_as(e + i, v[i]);
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) reinterpret_cast<uint4 *>(p)[i] = raw[i];
+}
+
 template <class TY, class TO>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kCombineThreads)
 combine_pairs_kernel(const TY *y, size_t ld_y, int n_y_rows, const int *pair_row, const float *w, int top_k, int cols, const TO *residual,
-                     size_t ld_residual, TO *out, size_t ld_out) {
+                     size_t ld_residual, TO *out, size_t ld_out, int vec) {
+  grid_dep_sync();
   const size_t t = blockIdx.x;
-  for (int c = threadIdx.x; c < cols; c += blockDim.x) {
-    float sum = 0.f;
-    for (int k = 0; k < top_k; ++k) {
-      const int r = pair_row[t * top_k + k];
-      if (r >= 0 && r < n_y_rows) sum = fmaf(w[t * top_k + k], to_f32(y[static_cast<size_t>(r) * ld_y + c]), sum);
+  const int *rows = pair_row + t * top_k;
+  const float *weights = w + t * top_k;
+  const int first = (blockIdx.y * blockDim.x + threadIdx.x) * kCombineCols, step = gridDim.y * blockDim.x * kCombineCols;
+  const int whole = vec ? cols / kCombineCols * kCombineCols : 0;   // columns that are read and written in vectors
+  constexpr int kAhead = 4;
+  // the first four pairs: their rows' vectors of the next step are on their way while those of this step are added
+  const TY *src[kAhead];
+  float f[kAhead];
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k) {
+    const int r = k < top_k ? rows[k] : -1;
+    const bool on = r >= 0 && r < n_y_rows;
+    src[k] = on ? y + static_cast<size_t>(r) * ld_y : nullptr;
+    f[k] = on ? weights[k] : 0.f;
+  }
+  Raw8<TY> v[kAhead];
+  Raw8<TO> res;
+  auto fetch = [&](int c0) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (src[k] != nullptr) v[k].load(src[k] + c0);
+    if (residual != nullptr) res.load(residual + t * ld_residual + c0);
+  };
+  int c0 = first;
+  if (c0 < whole) fetch(c0);
+  for (; c0 < whole; c0 += step) {
+    float sum[8] = {}, plus[8] = {};
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (src[k] != nullptr) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum[i] = fmaf(f[k], v[k][i], sum[i]);
+      }
+    if (residual != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) plus[i] = res[i];
     }
-    if (residual != nullptr) sum += to_f32(residual[t * ld_residual + c]);
-    store_as(out + t * ld_out + c, sum);
+    if (c0 + step < whole) fetch(c0 + step);
+    for (int k = kAhead; k < top_k; ++k) {
+      const int r = rows[k];
+      if (r < 0 || r >= n_y_rows) continue;
+      Raw8<TY> u;
+      u.load(y + static_cast<size_t>(r) * ld_y + c0);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[i] = fmaf(weights[k], u[i], sum[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum[i] += plus[i];
+    store8(out + t * ld_out + c0, sum);
+  }
+  for (; c0 < cols; c0 += step) {
+    float sum[8] = {};
+    for (int k = 0; k < top_k; ++k) {
+      const int r = rows[k];
+      if (r < 0 || r >= n_y_rows) continue;
+      const TY *from = y + static_cast<size_t>(r) * ld_y + c0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c0 + i < cols) sum[i] = fmaf(weights[k], to_f32(from[i]), sum[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c0 + i < cols) store_as(out + t * ld_out + c0 + i, residual != nullptr ? sum[i] + to_f32(residual[t * ld_residual + c0 + i]) : sum[i]);
   }
 }
 
 template <class TY, class TO>
 cudaError_t launch_combine_pairs(const void *y, size_t ld_y, int n_y_rows, const int *pair_row, const float *w, int rows, int top_k, int cols,
                                  const void *residual, size_t ld_residual, void *out, size_t ld_out, cudaStream_t s) {
-  combine_pairs_kernel<TY, TO><<<rows, 256, 0, s>>>(static_cast<const TY *>(y), ld_y, n_y_rows, pair_row, w, top_k, cols,
-                                                    static_cast<const TO *>(residual), ld_residual, static_cast<TO *>(out), ld_out);
-  return cudaGetLastError();
+  const int vec = aligned_to(y, 16) && aligned_to(residual, 16) && aligned_to(out, 16) && ld_y * sizeof(TY) % 16 == 0 &&
+                  ld_residual * sizeof(TO) % 16 == 0 && ld_out * sizeof(TO) % 16 == 0;
+  const int vectors = (cols + kCombineCols - 1) / kCombineCols;
+  const int parts = rows >= 1024 ? 1 : (vectors + kCombineThreads - 1) / kCombineThreads;
+  const int steps = (vectors + kCombineThreads * parts - 1) / (kCombineThreads * parts);
+  const int threads = ((vectors + steps * parts - 1) / (steps * parts) + 31) / 32 * 32;
+  const dim3 grid(rows, parts, 1);
+  return launch_kernel(combine_pairs_kernel<TY, TO>, grid, threads, 0, s, true, 0, static_cast<const TY *>(y), ld_y, n_y_rows, pair_row, w,
+                       top_k, cols, static_cast<const TO *>(residual), ld_residual, static_cast<TO *>(out), ld_out, vec);
 }
 
 }  // namespace moe
@@ -286,13 +567,13 @@ int moe_group_pairs(moe_handle c, const int *idx_dev, int rows, int top_k, int n
   if (!aligned_to(idx_dev, 4) || !aligned_to(offsets_dev, 4) || !aligned_to(pair_row_dev, 4) || !aligned_to(row_pair_dev, 4))
     return op_fail(c, MOE_ERR_INVALID, "moe_group_pairs: a tensor is not aligned to its elements");
   if (int rc = use_device(c, "moe_group_pairs")) return rc;
-  const size_t smem = static_cast<size_t>(kGroupWarps) * n_experts * sizeof(int);
-  cudaError_t e = allow_smem(c, reinterpret_cast<const void *>(group_pairs_kernel), kGroupWarps * kMaxGroupedExperts * 4, kSmemGroup);
-  if (e == cudaSuccess) {
-    group_pairs_kernel<<<1, kGroupThreads, smem, static_cast<cudaStream_t>(stream)>>>(idx_dev, static_cast<size_t>(rows) * top_k, n_experts,
-                                                                                      offsets_dev, pair_row_dev, row_pair_dev);
-    e = cudaGetLastError();
-  }
+  const size_t smem = static_cast<size_t>(kGroupWarps + 1) * n_experts * sizeof(int), n_pairs = static_cast<size_t>(rows) * top_k;
+  int ctas = 1;   // one step of 32 pairs for every warp, then more steps
+  while (ctas < kGroupMaxCtas && n_pairs > static_cast<size_t>(ctas) * kGroupThreads) ctas *= 2;
+  cudaError_t e = allow_smem(c, reinterpret_cast<const void *>(group_pairs_kernel), (kGroupWarps + 1) * kMaxGroupedExperts * 4, kSmemGroup);
+  if (e == cudaSuccess)
+    e = launch_kernel(group_pairs_kernel, dim3(1, ctas, 1), kGroupThreads, smem, static_cast<cudaStream_t>(stream), true, ctas > 1 ? ctas : 0, idx_dev,
+                      n_pairs, n_experts, offsets_dev, pair_row_dev, row_pair_dev);
   return launched(c, "moe_group_pairs", e);
 }
 
@@ -301,7 +582,7 @@ int moe_combine_pairs(moe_handle c, const void *y_dev, int y_dtype, long long ld
                       long long ld_out, void *stream) {
   if (!c) return MOE_ERR_INVALID;
   const int ys = dtype_size(y_dtype), os = dtype_size(out_dtype);
-  if (!ys || !os || rows < 0 || top_k < 1 || cols < 1 || n_y_rows < 0 || ld_y < cols || ld_out < cols || (residual_dev && ld_residual < cols) ||
+  if (!ys || !os || rows < 0 || top_k < 1 || cols < 1 || n_y_rows < 0 || cols > 65535 * kCombineThreads * kCombineCols || ld_y < cols || ld_out < cols || (residual_dev && ld_residual < cols) ||
       static_cast<long long>(rows) * top_k > 0x7fffffffll)
     return op_fail(c, MOE_ERR_INVALID, "moe_combine_pairs: dtypes %d and %d, %d rows x %d of %d columns, strides %lld, %lld, %lld", y_dtype, out_dtype,
                    rows, top_k, cols, ld_y, ld_residual, ld_out);

@@ -53,9 +53,9 @@ __device__ __forceinline__ uint32_t map_to_cta(uint32_t saddr, uint32_t cta) {
 __device__ __forceinline__ void mbar_arrive_relaxed_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {   // addr: from map_to_cta
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {   // addr: from map_to_cta
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
 }
 __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
