@@ -59,7 +59,7 @@ __device__ __forceinline__ R warp_sum(R v) {
 // expert (or -1) in `sel`.  R = float: returns false where 32 bits do not settle a comparison.  `top` and `sum`: of the softmax.
 // `group_lanes`: lanes of a group, where groups are runs of whole lanes, a power of two of them; else 0 and `shared` is used.
 template <class R, int kPer>
-__device__ __forceinline__ bool select_experts(const float (&x)[kPer], const float *bias, const moe_route_rule &rule, int per_lane, int group_lanes,
+__device__ __forceinline__ bool select_experts(const float (&x)[kPer], const float (&b)[kPer], const moe_route_rule &rule, int per_lane, int group_lanes,
                                                unsigned long long *shared, int lane, float top, double &sum, int &sel, R &sel_s) {
   constexpr bool kFast = sizeof(R) == 4;
   using Key = decltype(ordered_key(R()));
@@ -97,12 +97,9 @@ __device__ __forceinline__ bool select_experts(const float (&x)[kPer], const flo
     return va - vb > twice * (close + rel * (fabs(va) + fabs(vb)));
   };
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    key[i] = 0;
-    if (i < per_lane && x[i] > -inf) {
-      const float b = bias != nullptr ? bias[first + i] : 0.f;
-      if (b > -inf) key[i] = ordered_key(s[i] + static_cast<R>(b));
-    }
+  for (int i = 0; i < kPer; ++i) {   // (b: -inf where the lane has no expert)
+    key[i] = ordered_key(s[i] + static_cast<R>(b[i]));
+    if (!(x[i] > -inf) || !(b[i] > -inf)) key[i] = 0;
   }
   bool settled = true;
   if (rule.n_groups > 1) {
@@ -148,55 +145,69 @@ __device__ __forceinline__ bool select_experts(const float (&x)[kPer], const flo
       const Key a = __shfl_sync(0xffffffffu, worth, __ffs(in) - 1), b = __shfl_sync(0xffffffffu, worth, __ffs(out) - 1);
       if (b != 0 && !certain(a, b, R(2))) settled = false;
     }
+    if (kFast || group_lanes > 0) {
+      if (!(stays >> (lane / group_lanes) & 1u)) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (i < per_lane && first + i < rule.n_experts && !(stays >> ((first + i) / size) & 1u)) key[i] = 0;
+        for (int i = 0; i < kPer; ++i) key[i] = 0;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (i < per_lane && first + i < rule.n_experts && !(stays >> ((first + i) / size) & 1u)) key[i] = 0;
+    }
   }
-  // rounds: the largest key of a lane, then of the warp; the lowest lane of equal ones.  In 32 bits one round more, for the
-  // first that is not selected.
+  // rounds: the largest key of a lane, then of the warp; the lowest lane of equal ones, and in it the lowest expert.  In 32 bits
+  // one round more, for the first that is not selected: lane k keeps the k-th key, and neighbours are compared at the end.
   sel = -1;
   sel_s = 0;
-  Key best = 0, last = 0;
-  int at = 0;
-  auto find = [&]() {
-    best = key[0];
-    at = 0;
+  Key best = key[0], kept = 0;
 #pragma unroll
-    for (int i = 1; i < kPer; ++i)
-      if (key[i] > best) { best = key[i]; at = i; }
-  };
-  find();
-  for (int k = 0; k < rule.top_k + (kFast ? 1 : 0); ++k) {
+  for (int i = 1; i < kPer; ++i) best = max(best, key[i]);
+  const int rounds = rule.top_k + (kFast ? 1 : 0);
+  Key beyond = 0;   // of the round that has no lane
+  for (int k = 0; k < rounds; ++k) {
     unsigned owners;
     const Key top_key = warp_best(best, owners);
     if (top_key == 0) break;   // nothing left
-    if (kFast && k > 0 && !certain(last, top_key, R(1))) settled = false;
-    if (kFast && (__popc(owners) > 1 || !settled)) { settled = false; break; }
-    last = top_key;
-    const int owner = __ffs(owners) - 1, e = __shfl_sync(0xffffffffu, first + at, owner);
-    if (lane == k && k < rule.top_k) sel = e;
-    if (!kFast) {
-      R es = 0;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (i == at) es = s[i];
-      es = __shfl_sync(0xffffffffu, es, owner);
-      if (lane == k) sel_s = es;
-    }
+    if (lane == k) kept = top_key;
+    if (k == 32) beyond = top_key;
+    if (kFast && k == rule.top_k) break;
+    const int owner = __ffs(owners) - 1;
+    int e = 0;
+    R es = 0;
     if (lane == owner) {
+      Key next = 0;
+      bool found = false;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (i == at) key[i] = 0;
-      find();
+      for (int i = 0; i < kPer; ++i) {
+        const bool hit = !found && key[i] == top_key;
+        if (hit) {
+          e = first + i;
+          if (!kFast) es = s[i];
+          key[i] = 0;
+        }
+        found = found || hit;
+        next = max(next, key[i]);
+      }
+      best = next;
     }
+    e = __shfl_sync(0xffffffffu, e, owner);
+    if (!kFast) es = __shfl_sync(0xffffffffu, es, owner);
+    if (lane == k) { sel = e; sel_s = es; }
+  }
+  if (kFast) {
+    Key after = __shfl_down_sync(0xffffffffu, kept, 1);
+    if (lane == 31) after = beyond;
+    const bool close_call = lane < rule.top_k && kept != 0 && after != 0 && !certain(kept, after, R(1));
+    if (__any_sync(0xffffffffu, close_call)) settled = false;
   }
   return settled;
 }
 
 template <class T, int kPer>
 __global__ void __launch_bounds__(kRouteWarps * 32)
-route_scored_kernel(const T *logits, size_t ld, const float *bias, int rows, moe_route_rule rule, int per_lane, int group_lanes, int vec, int *idx,
-                    float *w) {
+route_scored_kernel(const T *logits, size_t ld, const float *bias, int rows, moe_route_rule rule, int per_lane, int group_lanes, int vec, int vec_bias,
+                    int *idx, float *w) {
   __shared__ unsigned long long s_keys[kRouteWarps][kPer * 32];   // groups that are not whole lanes
   grid_dep_sync();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -223,6 +234,23 @@ route_scored_kernel(const T *logits, size_t ld, const float *bias, int rows, moe
     for (int i = 0; i < kPer; ++i)
       if (i < per_lane && first + i < E) x[i] = to_f32(src[first + i]);
   }
+  float b[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) b[i] = i < per_lane && first + i < E ? 0.f : -inf;
+  if (bias != nullptr) {
+    if (kPer >= 4 && vec_bias) {
+#pragma unroll
+      for (int i = 0; i + 4 <= kPer; i += 4)
+        if (i < per_lane && first + i < E) {
+          const float4 v = *reinterpret_cast<const float4 *>(bias + first + i);
+          b[i] = v.x; b[i + 1] = v.y; b[i + 2] = v.z; b[i + 3] = v.w;
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (i < per_lane && first + i < E) b[i] = bias[first + i];
+    }
+  }
   float top = -inf;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
@@ -239,7 +267,7 @@ route_scored_kernel(const T *logits, size_t ld, const float *bias, int rows, moe
   double sum = 0.0, share = 0.0;
   float unused;
   if ((rule.n_groups == 1 || group_lanes > 0) &&
-      select_experts<float, kPer>(x, bias, rule, per_lane, group_lanes, nullptr, lane, top, sum, sel, unused)) {
+      select_experts<float, kPer>(x, b, rule, per_lane, group_lanes, nullptr, lane, top, sum, sel, unused)) {
     // weights of the selected from their logits, within a few roundings of 32 bits
     float s = 0.f;
     if (sel >= 0) {
@@ -261,7 +289,7 @@ route_scored_kernel(const T *logits, size_t ld, const float *bias, int rows, moe
     }
   } else {
     double s;
-    select_experts<double, kPer>(x, bias, rule, per_lane, group_lanes, s_keys[warp], lane, top, sum, sel, s);
+    select_experts<double, kPer>(x, b, rule, per_lane, group_lanes, s_keys[warp], lane, top, sum, sel, s);
     share = s;
     if (rule.renormalise) {
       const double all = warp_sum(s);
@@ -288,8 +316,9 @@ cudaError_t launch_route_scored(const moe_route_rule &r, const void *logits, siz
   const T *x = static_cast<const T *>(logits);
   constexpr int kVec = 16 / static_cast<int>(sizeof(T));
   const int vec = per % kVec == 0 && r.n_experts % kVec == 0 && ld % kVec == 0 && aligned_to(x, 16);
+  const int vec_bias = per % 4 == 0 && r.n_experts % 4 == 0 && aligned_to(bias, 16);
   auto go = [&](auto kernel) {
-    return launch_kernel(kernel, dim3(grid), kRouteWarps * 32, 0, s, true, 0, x, ld, bias, rows, r, per, group_lanes, vec, idx, w);
+    return launch_kernel(kernel, dim3(grid), kRouteWarps * 32, 0, s, true, 0, x, ld, bias, rows, r, per, group_lanes, vec, vec_bias, idx, w);
   };
   if (per <= 1) return go(route_scored_kernel<T, 1>);
   if (per <= 2) return go(route_scored_kernel<T, 2>);
@@ -311,7 +340,7 @@ constexpr int kMaxGroupedExperts = 1024;
 __global__ void __launch_bounds__(kGroupThreads)
 group_pairs_kernel(const int *idx, size_t n_pairs, int E, int *offsets, int *pair_row, int *row_pair) {
   extern __shared__ int s_hist[];   // [kGroupWarps][E], then the totals of this CTA [E]
-  __shared__ int s_scan[kGroupWarps], s_all;
+  __shared__ int s_scan[kGroupWarps], s_all, s_start[kMaxGroupedExperts];   // s_start: first row of this CTA's pairs of an expert
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int ctas = gridDim.y, rank = blockIdx.y;   // the cluster is the grid
   int *mine = s_hist + warp * E, *totals = s_hist + kGroupWarps * E;
@@ -340,10 +369,13 @@ group_pairs_kernel(const int *idx, size_t n_pairs, int E, int *offsets, int *pai
   // thread e: exclusive prefix over the warps of this CTA, then over the CTAs and the experts
   int total = 0;
   if (threadIdx.x < E) {
+    int n[kGroupWarps];
+#pragma unroll
+    for (int v = 0; v < kGroupWarps; ++v) n[v] = s_hist[v * E + threadIdx.x];
+#pragma unroll
     for (int v = 0; v < kGroupWarps; ++v) {
-      const int n = s_hist[v * E + threadIdx.x];
       s_hist[v * E + threadIdx.x] = total;
-      total += n;
+      total += n[v];
     }
     totals[threadIdx.x] = total;
   }
@@ -380,17 +412,24 @@ group_pairs_kernel(const int *idx, size_t n_pairs, int E, int *offsets, int *pai
   const int start = s_scan[warp] + incl - all;
   if (threadIdx.x < E) {
     if (rank == 0) offsets[threadIdx.x] = start;
-    for (int v = 0; v < kGroupWarps; ++v) s_hist[v * E + threadIdx.x] += start + before;
+    s_start[threadIdx.x] = start + before;
   }
   if (rank == 0 && threadIdx.x == 0) offsets[E] = s_all;
   __syncthreads();
+  // lanes with the same expert, from a ballot for each bit of its number (__match_any_sync takes ~60 cycles for every distinct
+  // number of the warp: 2000 a step with 256 experts, 14 of the 22 us that the call took)
+  const int bits = 32 - __clz(E);
   auto place = [&](size_t p, int e) {
-    const unsigned same = __match_any_sync(0xffffffffu, e);
+    unsigned same = __ballot_sync(0xffffffffu, e >= 0);
+    for (int i = 0; i < bits; ++i) {
+      const unsigned set = __ballot_sync(0xffffffffu, e >> i & 1);
+      same &= (e >> i & 1) ? set : ~set;
+    }
     const int rank_here = __popc(same & ((1u << lane) - 1u));
     int row = -1;
-    if (e >= 0) row = mine[e] + rank_here;
+    if (e >= 0) row = s_start[e] + mine[e] + rank_here;
     __syncwarp();
-    if (e >= 0 && rank_here == 0) mine[e] += __popc(same);
+    if (e >= 0 && rank_here == 0) mine[e] += __popc(same);   // one lane of each expert
     __syncwarp();
     if (p < end) pair_row[p] = row;
     if (row >= 0 && row_pair != nullptr) row_pair[row] = static_cast<int>(p);
