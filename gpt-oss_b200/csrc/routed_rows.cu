@@ -13,9 +13,11 @@ namespace moe {
 // lower index;  weight = s [/ sum of the selected s] * scale.  An expert is off where x or its bias is -inf or NaN.
 //
 // Which of two neighbouring p is larger is part of the answer, so the comparisons are those of 64 bits.  A row is tried in
-// 32 bits first: there an s is off by less than 2^-18 of the row's largest possible s (exp, a sum of up to 512, a quotient), so
-// an order is certain where the two values differ by 2^-17 of it and 2^-22 of their own magnitudes (twice that for sums of two).
-// A row with a closer call (equal scores, scores that saturate) is done again in 64 bits.
+// 32 bits first.  There a sigmoid is off by less than 2^-21 (s (1 - s) times the exponential's (2 + 1.2 |x|) 2^-23, and the
+// roundings of sum and quotient), a softmax by less than 2^-18 of the row's largest (exponentials, a sum of up to 512, a quotient);
+// so an order is certain where two values differ by 2^-20, or 2^-17 of that largest, and 2^-22 of their own magnitudes (twice
+// that for sums of two).  A row with a closer call (equal scores, scores that saturate) is done again in 64 bits: 4 us more for a
+// call of 8192 rows in which one row in a hundred is, however few.
 //
 // A warp per row; lane l owns the per_lane consecutive experts from l * per_lane, so that a lower lane is a lower index.
 // ---------------------------------------------------------------------------
@@ -91,7 +93,8 @@ __device__ __forceinline__ bool select_experts(const float (&x)[kPer], const flo
       else s[i] = 1.0 / (1.0 + exp(-static_cast<double>(x[i])));
     }
   }
-  const R close = bound * R(7.62939453125e-06), rel = R(2.384185791015625e-07);   // 2^-17, 2^-22
+  const R close = rule.score == MOE_SCORE_SOFTMAX ? bound * R(7.62939453125e-06) : R(9.5367431640625e-07);   // 2^-17, 2^-20
+  const R rel = R(2.384185791015625e-07);   // 2^-22
   auto certain = [&](Key a, Key b, R twice) {   // a is the larger of two keys that are on
     const R va = key_value(a), vb = key_value(b);
     return va - vb > twice * (close + rel * (fabs(va) + fabs(vb)));
