@@ -26,6 +26,8 @@ inline bool aligned_to(const void *p, size_t n) { return (reinterpret_cast<uintp
 
 // Makes the handle's device current; every entry calls it after its own checks.
 inline int use_device(moe_ctx *c, const char *who) {
+  int current = -1;
+  if (cudaGetDevice(&current) == cudaSuccess && current == c->cfg.device) return MOE_OK;
   const cudaError_t e = cudaSetDevice(c->cfg.device);
   return e == cudaSuccess ? MOE_OK : op_fail(c, MOE_ERR_CUDA, "%s: cudaSetDevice(%d): %s", who, c->cfg.device, cudaGetErrorString(e));
 }
