@@ -89,25 +89,65 @@ __device__ __forceinline__ void store_out(const Fp8GemmArgs &p, size_t at, float
   else store_as(static_cast<float *>(p.out) + at, v);
 }
 
-// Four neighbouring sums of a tile whose reduction is split: the parts of all CTAs of the cluster, requested together and added
-// in the order of k.
-constexpr int kMaxSplits = 4;
-__device__ __forceinline__ float4 sum_of_splits(uint32_t at, int splits) {
-  float4 v[kMaxSplits];
-#pragma unroll
-  for (int r = 0; r < kMaxSplits; ++r)
-    if (r < splits) v[r] = ld_cluster_f32x4(map_to_cta(at, r));
-  float4 sum = v[0];
-#pragma unroll
-  for (int r = 1; r < kMaxSplits; ++r)
-    if (r < splits) { sum.x += v[r].x; sum.y += v[r].y; sum.z += v[r].z; sum.w += v[r].w; }
-  return sum;
+// Two neighbouring 16-bit outputs, of which `left` exist, where rows are aligned to `bytes`.
+__device__ __forceinline__ void store_word16(uint16_t *dst, uint32_t w, int left, int bytes) {
+  if (left >= 2 && bytes >= 4) {
+    *reinterpret_cast<uint32_t *>(dst) = w;
+  } else {
+    if (left >= 1) dst[0] = static_cast<uint16_t>(w);
+    if (left >= 2) dst[1] = static_cast<uint16_t>(w >> 16);
+  }
 }
+
+constexpr int kMaxSplits = 4;   // CTAs of a cluster that share the reduction of a tile
 
 // One tile: rows [row0, row0 + ntok) of group g against weight rows [128 nb, 128 nb + 128).
 struct GemmTile {
   int g, nb, row0, ntok;
 };
+
+// A CTA's share of a split tile, kWidth output columns from n0: rows split, split + splits, ..., `mine` of them.  Four places of a
+// thread are under way together: a load from another CTA's shared memory takes about a microsecond.
+template <int kWidth, int kThreads>
+__device__ __forceinline__ void add_up_splits(const Fp8GemmArgs &p, const GemmTile &t, uint32_t part, int pitch, int mine, int split, int n0, int out_bytes) {
+  constexpr int kQuads = kWidth / 4, kAhead = 4;
+  for (int e0 = threadIdx.x; e0 < mine * kQuads; e0 += kAhead * kThreads) {
+    float4 v[kAhead][kMaxSplits];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int e = e0 + i * kThreads;
+#pragma unroll
+      for (int r = 0; r < kMaxSplits; ++r)
+        if (e < mine * kQuads && r < p.splits)
+          v[i][r] = ld_cluster_f32x4(map_to_cta(part + 4u * ((split + e / kQuads * p.splits) * pitch + e % kQuads * 4), r));
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int e = e0 + i * kThreads, row = split + e / kQuads * p.splits, n = n0 + e % kQuads * 4;
+      if (e >= mine * kQuads) break;
+      float4 sum = v[i][0];
+#pragma unroll
+      for (int r = 1; r < kMaxSplits; ++r)
+        if (r < p.splits) { sum.x += v[i][r].x; sum.y += v[i][r].y; sum.z += v[i][r].z; sum.w += v[i][r].w; }   // in the order of k
+      float o[4] = {sum.x, sum.y, sum.z, sum.w};
+      if (p.bias != nullptr) {
+        const __nv_bfloat16 *bias = p.bias + static_cast<size_t>(t.g) * p.n + n;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] += n + j < p.n ? __bfloat162float(bias[j]) : 0.f;
+      }
+      const size_t at = static_cast<size_t>(t.row0 + row) * p.ld_out + n;
+      if (out_bytes == 16 && n + 4 <= p.n) {
+        if (p.out_dtype == MOE_F32) *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at) = make_float4(o[0], o[1], o[2], o[3]);
+        else if (p.out_dtype == MOE_BF16) *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + at) = make_uint2(pack2<__nv_bfloat16>(o[0], o[1]), pack2<__nv_bfloat16>(o[2], o[3]));
+        else *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + at) = make_uint2(pack2<__half>(o[0], o[1]), pack2<__half>(o[2], o[3]));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n + j < p.n) store_out(p, at + j, o[j]);
+      }
+    }
+  }
+}
 
 // Offsets that are not ascending give wrong rows, never rows outside.
 __device__ __forceinline__ int group_begin(const Fp8GemmArgs &p, int g) { return p.offsets == nullptr ? 0 : min(max(p.offsets[g], 0), p.rows); }
@@ -153,7 +193,7 @@ __device__ __forceinline__ GemmTile tile_at(const Fp8GemmArgs &p, const int *s_t
 
 template <int kTok>
 __global__ void __launch_bounds__(GemmShape<kTok>::kThreads, 1)
-fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const Fp8GemmArgs p, const int wide_out) {
+fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const Fp8GemmArgs p, const int out_bytes) {
   using S = GemmShape<kTok>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ int s_tiles[kMaxGemmGroups + 1];   // token tiles of the groups before g
@@ -378,12 +418,12 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
       __syncwarp();
       if (lane == 0) mbar_arrive(pempty(plan));
       if (plan ^= 1u; plan == 0) ppar ^= 1u;
-      if (wide_out) {
-        // 16-bit outputs: blocks of 8 tokens x 32 weight rows are transposed in shared memory and leave as 16 bytes a lane
+      if (p.out_dtype != MOE_F32) {
+        // 16-bit outputs: blocks of 8 tokens x 32 weight rows are transposed in shared memory and leave as 16 bytes a lane (out_bytes),
+        // or as the 4 or 2 that the output's rows are aligned to
         const uint32_t stage = ring + S::kOutOff + warp * S::kOutWarp;
-        const uint32_t st_at = stage + (lane & 7) * S::kOutPitch + (lane >> 3) * 16, ld_at = stage + (lane >> 2) * S::kOutPitch + (lane & 3) * 16;
-        const int n = n_w + (lane & 3) * 8, ntok = t.ntok - col0;
-        uint16_t *dst = static_cast<uint16_t *>(p.out) + static_cast<size_t>(t.row0 + col0 + (lane >> 2)) * p.ld_out + n;
+        const uint32_t st_at = stage + (lane & 7) * S::kOutPitch + (lane >> 3) * 16;
+        const int ntok = t.ntok - col0;
 #pragma unroll
         for (int j0 = 0; j0 < S::kCols / 8; j0 += S::kOutCols / 8) {
           if (8 * j0 >= ntok) break;
@@ -400,17 +440,28 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
             stmatrix_trans_x4(st_at + j * 8 * S::kOutPitch, w[0], w[1], w[2], w[3]);
           }
           __syncwarp();
+          uint16_t *out = static_cast<uint16_t *>(p.out) + static_cast<size_t>(t.row0 + col0 + 8 * j0) * p.ld_out + n_w;
+          const int here = min(ntok - 8 * j0, S::kOutCols);
+          if (out_bytes == 16) {
+            const int n = (lane & 3) * 8;
+            for (int tok = lane >> 2; tok < here; tok += 8) {
+              uint32_t o[4];
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]) : "r"(stage + tok * S::kOutPitch + n * 2) : "memory");
+              uint16_t *dst = out + static_cast<size_t>(tok) * p.ld_out + n;
+              if (n_w + n + 8 <= p.n) {
+                *reinterpret_cast<uint4 *>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+              } else {
 #pragma unroll
-          for (int j = 0; j < S::kOutCols / 8; ++j, dst += 8 * p.ld_out) {
-            if (8 * (j0 + j) + (lane >> 2) >= ntok || n >= p.n) continue;
-            uint32_t o[4];
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]) : "r"(ld_at + j * 8 * S::kOutPitch) : "memory");
-            if (n + 8 <= p.n) {
-              *reinterpret_cast<uint4 *>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
-            } else {
-#pragma unroll
-              for (int e = 0; e < 8; ++e)
-                if (n + e < p.n) dst[e] = static_cast<uint16_t>(o[e / 2] >> (16 * (e & 1)));
+                for (int e = 0; e < 8; ++e)
+                  if (n_w + n + e < p.n) dst[e] = static_cast<uint16_t>(o[e / 2] >> (16 * (e & 1)));
+              }
+            }
+          } else {
+            const int n = (lane & 15) * 2;
+            for (int tok = lane >> 4; tok < here; tok += 2) {
+              uint32_t o;
+              asm volatile("ld.shared.b32 %0, [%1];" : "=r"(o) : "r"(stage + tok * S::kOutPitch + n * 2) : "memory");
+              store_word16(out + static_cast<size_t>(tok) * p.ld_out + n, o, p.n - n_w - n, out_bytes);
             }
           }
         }
@@ -436,15 +487,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
       const GemmTile t = tile_of(it);
       const uint32_t base = smem_u32(ring_ptr);
       const int mine = (t.ntok - split + p.splits - 1) / p.splits;
-      for (int e = threadIdx.x; e < mine * (kScaleBlock / 4); e += S::kThreads) {
-        const int tok = split + e / (kScaleBlock / 4) * p.splits, r = e % (kScaleBlock / 4) * 4, n = t.nb * kScaleBlock + r;
-        const float4 sum = sum_of_splits(base + 4u * (tok * S::kPartPitch + r), p.splits);
-        const float o[4] = {sum.x, sum.y, sum.z, sum.w};
-        const size_t at = static_cast<size_t>(t.row0 + tok) * p.ld_out + n;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (n + i < p.n) store_out(p, at + i, o[i] + (p.bias != nullptr ? __bfloat162float(p.bias[static_cast<size_t>(t.g) * p.n + n + i]) : 0.f));
-      }
+      add_up_splits<kScaleBlock, S::kThreads>(p, t, base, S::kPartPitch, mine, split, t.nb * kScaleBlock, out_bytes);
     }
     cluster_sync_all();   // no CTA leaves while another may still read its part
   }
@@ -481,24 +524,40 @@ static_assert(kWideCols == kScaleBlock, "one sb per warp and block of k");
 static_assert(kWideTok * kWidePart * 4 <= kWideStages * kWideStage, "a split's partial tile reuses the ring");
 static_assert(kWideSmem + 4608 <= 227 * 1024, "shared memory");
 
-// What the copy engine would do with a box of staged outputs (128-byte swizzle), by a warp: rows [0, rows) to output rows
-// row0.. and columns n..; 16 bytes a lane where the output is aligned for it, else an element.
-__device__ __forceinline__ void copy_box(const Fp8GemmArgs &p, const uint8_t *box, int row0, int rows, int n) {
+// What the copy engine would do with a box of staged outputs (128-byte swizzle), by a warp: rows [0, rows) to output rows row0..
+// and columns n..; 16 bytes a lane where the output's rows are aligned to that, else 4 or 2.
+__device__ __forceinline__ void copy_box(const Fp8GemmArgs &p, const uint8_t *box, int row0, int rows, int n, int out_bytes) {
   const int lane = threadIdx.x & 31, size = p.out_dtype == MOE_F32 ? 4 : 2, per = 16 / size;
-  const bool wide = (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0 && p.ld_out % per == 0;
-  for (int i = lane; i < rows * 8; i += 32) {   // (row, 16-byte piece)
-    const int r = i / 8, piece = i % 8, col = n + piece * per;
-    const uint4 v = *reinterpret_cast<const uint4 *>(box + r * 128 + ((piece ^ (r & 7)) << 4));
-    const size_t at = static_cast<size_t>(row0 + r) * p.ld_out + col;
-    if (wide && col + per <= p.n) {
-      *reinterpret_cast<uint4 *>(static_cast<uint8_t *>(p.out) + at * size) = v;
-    } else {
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-      for (int j = 0; j < per; ++j) {
-        if (col + j >= p.n) break;
-        if (size == 4) static_cast<uint32_t *>(p.out)[at + j] = w[j];
-        else static_cast<uint16_t *>(p.out)[at + j] = static_cast<uint16_t>(w[j / 2] >> (16 * (j & 1)));
+  if (out_bytes == 16) {
+    for (int i = lane; i < rows * 8; i += 32) {   // (row, 16-byte piece)
+      const int r = i / 8, piece = i % 8, col = n + piece * per;
+      const uint4 v = *reinterpret_cast<const uint4 *>(box + r * 128 + ((piece ^ (r & 7)) << 4));
+      const size_t at = static_cast<size_t>(row0 + r) * p.ld_out + col;
+      if (col + per <= p.n) {
+        *reinterpret_cast<uint4 *>(static_cast<uint8_t *>(p.out) + at * size) = v;
+      } else {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (j >= per || col + j >= p.n) break;
+          if (size == 4) static_cast<uint32_t *>(p.out)[at + j] = w[j & 3];
+          else static_cast<uint16_t *>(p.out)[at + j] = static_cast<uint16_t>(w[j / 2] >> (16 * (j & 1)));
+        }
       }
+    }
+    return;
+  }
+  const int col = n + lane * 4 / size;   // a 4-byte word a lane, eight rows at a time
+  for (int r0 = 0; r0 < rows; r0 += 8) {
+    uint32_t w[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) w[r] = *reinterpret_cast<const uint32_t *>(box + (r0 + r) * 128 + ((lane / 4 ^ r) << 4) + lane % 4 * 4);
+    size_t at = static_cast<size_t>(row0 + r0) * p.ld_out + col;
+#pragma unroll
+    for (int r = 0; r < 8; ++r, at += p.ld_out) {
+      if (r0 + r >= rows) break;
+      if (size == 2) store_word16(static_cast<uint16_t *>(p.out) + at, w[r], p.n - col, out_bytes);
+      else if (col < p.n) static_cast<uint32_t *>(p.out)[at] = w[r];
     }
   }
 }
@@ -507,7 +566,7 @@ __device__ __forceinline__ void copy_box(const Fp8GemmArgs &p, const uint8_t *bo
 template <bool kSplit>
 __global__ void __launch_bounds__(kWideThreads, 1)
 fp8_gemm_wide_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_out,
-                     const Fp8GemmArgs p, const int tiled_out) {
+                     const Fp8GemmArgs p, const int tiled_out, const int out_bytes) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ int s_tiles[kMaxGemmGroups + 1];
   __shared__ uint32_t s_tmem, s_abort;
@@ -727,7 +786,7 @@ fp8_gemm_wide_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
             tma_store_commit();
           }
         } else {
-          copy_box(p, out_gen, row_out, min(rows_here, 32), n);
+          copy_box(p, out_gen, row_out, min(rows_here, 32), n, out_bytes);
         }
       };
       if (p.out_dtype == MOE_F32) {
@@ -762,15 +821,7 @@ fp8_gemm_wide_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
     if (first < n_items) {
       const GemmTile t = tile_at(p, s_tiles, first, n_nb);
       const int mine = (t.ntok - split + p.splits - 1) / p.splits;
-      for (int e = threadIdx.x; e < mine * (kWideN / 4); e += kWideThreads) {
-        const int row = split + e / (kWideN / 4) * p.splits, c = e % (kWideN / 4) * 4, n = t.nb * kWideN + c;
-        const float4 sum = sum_of_splits(ring + 4u * (row * kWidePart + c), p.splits);
-        const float o[4] = {sum.x, sum.y, sum.z, sum.w};
-        const size_t at = static_cast<size_t>(t.row0 + row) * p.ld_out + n;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (n + i < p.n) store_out(p, at + i, o[i] + (p.bias != nullptr ? __bfloat162float(p.bias[static_cast<size_t>(t.g) * p.n + n + i]) : 0.f));
-      }
+      add_up_splits<kWideN, kWideThreads>(p, t, ring, kWidePart, mine, split, t.nb * kWideN, out_bytes);
     }
     cluster_sync_all();   // no CTA leaves while another may still read its part
   }
@@ -810,6 +861,14 @@ bool encode_out(CUtensorMap *m, const Fp8GemmArgs &p) {
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Bytes that the output's rows are aligned to: 16, 4 or the size of an element.
+int out_alignment(const Fp8GemmArgs &p) {
+  const int size = dtype_size(p.out_dtype);
+  for (int bytes : {16, 4})
+    if (aligned_to(p.out, bytes) && p.ld_out * size % bytes == 0) return bytes;
+  return size;
+}
+
 struct GemmCall {
   const uint8_t *a, *b;
   long long ld_a, ld_b;
@@ -817,8 +876,9 @@ struct GemmCall {
   Fp8GemmArgs p;
 };
 
-// CTAs that share the reduction of a tile where the call has at most `tiles`: as many as keep all of them resident, each with
-// some blocks of k, in a cluster of the size that every device takes.
+// CTAs that share the reduction of a tile where the call has at most `tiles`: 1, 2 or 4, as many as leave no SM without one.
+// Clusters of three or eight do not all fit the device at once although their CTAs would: 393 x 3011 x 6502 (48 tiles) in two 32
+// us, in three 42; 16 rows x 4096 x 7168 (32 tiles of 64 columns) in four 9.3 us, in eight 20.
 int k_splits(long long tiles, int n_kb, int sm_count) {
   int splits = 1;
   while (splits < kMaxSplits && tiles * splits * 2 <= sm_count && splits * 2 <= n_kb) splits *= 2;
@@ -854,9 +914,8 @@ cudaError_t launch_fp8_gemm(moe_ctx *h, const GemmCall &c, cudaStream_t s, bool 
   const long long most = (groups + (c.p.rows - groups) / kTok) * n_nb;
   Fp8GemmArgs p = c.p;
   p.splits = k_splits(most, p.n_kb, sm_count);
-  const int wide = p.out_dtype != MOE_F32 && aligned_to(p.out, 16) && p.ld_out % 8 == 0;
   const dim3 grid(static_cast<unsigned>(p.splits > 1 ? most : std::min<long long>(most, sm_count)), p.splits, 1);
-  return launch_kernel(fp8_gemm_kernel<kTok>, grid, S::kThreads, S::kSmem, s, true, p.splits > 1 ? p.splits : 0, ma, mb, p, wide);
+  return launch_kernel(fp8_gemm_kernel<kTok>, grid, S::kThreads, S::kSmem, s, true, p.splits > 1 ? p.splits : 0, ma, mb, p, out_alignment(p));
 }
 
 cudaError_t launch_fp8_gemm_wide(moe_ctx *h, const GemmCall &c, cudaStream_t s, bool &maps_ok) {
@@ -873,9 +932,9 @@ cudaError_t launch_fp8_gemm_wide(moe_ctx *h, const GemmCall &c, cudaStream_t s, 
   if (e != cudaSuccess) return e;
   // outputs through the copy engine: rows of 16-byte pieces
   CUtensorMap mo = ma;
-  const int tiled = aligned_to(c.p.out, 16) && c.p.ld_out * dtype_size(c.p.out_dtype) % 16 == 0 && encode_out(&mo, c.p);
+  const int tiled = out_alignment(c.p) == 16 && encode_out(&mo, c.p);
   const dim3 grid(static_cast<unsigned>(p.splits > 1 ? most : std::min<long long>(most, sm_count)), p.splits, 1);
-  return launch_kernel(kernel, grid, kWideThreads, kWideSmem, s, true, p.splits > 1 ? p.splits : 0, ma, mb, mo, p, tiled);
+  return launch_kernel(kernel, grid, kWideThreads, kWideSmem, s, true, p.splits > 1 ? p.splits : 0, ma, mb, mo, p, tiled, out_alignment(p));
 }
 
 }  // namespace

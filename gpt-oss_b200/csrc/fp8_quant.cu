@@ -9,6 +9,8 @@
 // written at several places (the rows of a token's experts): the values are read and converted once.
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "fp8_layer.cuh"
 
 namespace moe {
@@ -65,31 +67,45 @@ __device__ __forceinline__ float gated(float gate, float up, float limit, float 
   return over_one_plus_exp2(gate, rate * gate) * up;
 }
 
-// Sixteen consecutive values of a row, of which `n` (any number) exist, as they lie in memory; wide: 16-byte loads.
+// Sixteen values of a row as they lie in memory: consecutive ones in 16-byte loads, or every eighth (eight lanes read neighbours).
+// `n`: how many columns there are from the first on.
 template <class T>
 struct Raw16 {
   uint4 v[sizeof(T)];
-  __device__ __forceinline__ void load(const T *p, int n, bool wide) {
-    if (wide && n >= 16) {
+  __device__ __forceinline__ void load(const T *p) {
 #pragma unroll
-      for (int i = 0; i < static_cast<int>(sizeof(T)); ++i) v[i] = reinterpret_cast<const uint4 *>(p)[i];
-    } else {
-      T *e = reinterpret_cast<T *>(v);
+    for (int i = 0; i < static_cast<int>(sizeof(T)); ++i) v[i] = reinterpret_cast<const uint4 *>(p)[i];
+  }
+  __device__ __forceinline__ void load_spread(const T *p, int n, int step) {
+    T *e = reinterpret_cast<T *>(v);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) e[i] = i < n ? p[i] : T(0.f);
-    }
+    for (int i = 0; i < 16; ++i) e[i] = kQuantLanes * i < n ? p[step * i] : T(0.f);
   }
   __device__ __forceinline__ float operator[](int i) const { return to_f32(reinterpret_cast<const T *>(v)[i]); }
 };
-__device__ __forceinline__ void write16(uint8_t *p, int n, bool wide, uint4 q) {
-  if (wide && n >= 16) {
-    *reinterpret_cast<uint4 *>(p) = q;
-  } else {
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+// Codes of every eighth column -> those of the lane's sixteen neighbours.  Bytes 2 m, 2 m + 1 of lane l are columns 16 m + l and
+// 16 m + 8 + l: an 8 x 8 transpose of byte pairs over the eight lanes.
+__device__ __forceinline__ uint4 gather_codes(uint4 q) {
+  const unsigned lane = threadIdx.x % kQuantLanes;
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  uint32_t lo[2] = {0, 0}, hi[2] = {0, 0};
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (i < n) p[i] = static_cast<uint8_t>(w[i / 4] >> (8 * (i & 3)));
+  for (unsigned step = 0; step < kQuantLanes; ++step) {
+    const unsigned other = lane ^ step;
+    const uint32_t pair_word = (other & 4) ? ((other & 2) ? w[3] : w[2]) : ((other & 2) ? w[1] : w[0]);
+    const uint32_t got = __shfl_xor_sync(0xffffffffu, pair_word >> (16 * (other & 1)), step);   // byte pair `lane` of lane `other`
+    const unsigned shift = 8 * (other & 3);
+    const uint32_t first = (got & 0xffu) << shift, second = ((got >> 8) & 0xffu) << shift;
+    if (other & 4) { lo[1] |= first; hi[1] |= second; }
+    else { lo[0] |= first; hi[0] |= second; }
   }
+  return make_uint4(lo[0], lo[1], hi[0], hi[1]);
+}
+__device__ __forceinline__ void write_spread(uint8_t *p, int n, uint4 q) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (kQuantLanes * i < n) p[kQuantLanes * i] = static_cast<uint8_t>(w[i / 4] >> (8 * (i & 3)));
 }
 __device__ __forceinline__ float finite_max(const float (&v)[16], float m) {
   float a = m;
@@ -108,10 +124,10 @@ __device__ __forceinline__ float finite_max(const float (&v)[16], float m) {
 // under way together cost registers and time.
 constexpr int kQuantThreads = 256, kQuantGroups = kQuantThreads / kQuantLanes, kPlaces = 4;
 
-template <class T, int kAct>
+template <class T, int kAct, bool kWideIn>
 __global__ void __launch_bounds__(kQuantThreads)
 quantize_fp8_kernel(const T *x, unsigned ld_x, int rows, int cols, unsigned n_blocks, float limit, float rate, const int *pair_row, unsigned fanout,
-                    int out_rows, const int *n_rows, uint8_t *codes, unsigned ld_codes, float *scales, unsigned ld_scales, int wide_in, int wide_out) {
+                    int out_rows, const int *n_rows, uint8_t *codes, unsigned ld_codes, float *scales, unsigned ld_scales, int wide_out) {
   grid_dep_sync();
   const unsigned lane = threadIdx.x % kQuantLanes;
   int live = rows;
@@ -122,7 +138,11 @@ quantize_fp8_kernel(const T *x, unsigned ld_x, int rows, int cols, unsigned n_bl
   for (unsigned unit = blockIdx.x * kQuantGroups + threadIdx.x / kQuantLanes; __any_sync(0xffffffffu, unit < units); unit += stride) {
     const bool on = unit < units;
     const unsigned row = on ? unit / n_blocks : 0, kb = on ? unit - row * n_blocks : n_blocks;   // no column of block n_blocks exists
-    const int c0 = static_cast<int>(kb * kScaleBlock + lane * kQuantCols), n = cols - c0;
+    // a lane's columns: sixteen neighbours, or, where rows of x are not 16-byte aligned and in a row's last part of a block, every
+    // eighth
+    const int left = cols - static_cast<int>(kb * kScaleBlock);
+    const bool whole = kWideIn && wide_out && left >= kScaleBlock;
+    const int c0 = static_cast<int>(kb * kScaleBlock + lane * (whole ? kQuantCols : 1)), n = cols - c0;
     const T *src = x + static_cast<size_t>(row) * ld_x;
     float v[16];
     int place[kPlaces];
@@ -133,31 +153,47 @@ quantize_fp8_kernel(const T *x, unsigned ld_x, int rows, int cols, unsigned n_bl
     }
     if (kAct == MOE_ACT_NONE) {
       Raw16<T> a;
-      a.load(src + c0, n, wide_in);
+      if (whole) a.load(src + c0);
+      else a.load_spread(src + c0, n, kQuantLanes);
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] = a[i];
-    } else if (kAct == MOE_ACT_SWIGLU) {
-      Raw16<T> a, b;
-      a.load(src + 2 * c0, 2 * n, wide_in);
-      b.load(src + 2 * c0 + 16, 2 * n - 16, wide_in);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[i] = gated<kAct>(a[2 * i], a[2 * i + 1], limit, rate);
-        v[i + 8] = gated<kAct>(b[2 * i], b[2 * i + 1], limit, rate);
-      }
     } else {
       Raw16<T> a, b;
-      a.load(src + c0, n, wide_in);
-      b.load(src + cols + c0, n, wide_in);
+      if (!whole) {   // gates in a, ups in b
+        const int at = kAct == MOE_ACT_SWIGLU ? 2 * c0 : c0, step = kAct == MOE_ACT_SWIGLU ? 2 * kQuantLanes : kQuantLanes;
+        a.load_spread(src + at, n, step);
+        b.load_spread(src + at + (kAct == MOE_ACT_SWIGLU ? 1 : cols), n, step);
+      } else if (kAct == MOE_ACT_SWIGLU) {
+        a.load(src + 2 * c0);
+        b.load(src + 2 * c0 + 16);
+      } else {
+        a.load(src + c0);
+        b.load(src + cols + c0);
+      }
+      if (kAct == MOE_ACT_SWIGLU && whole) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = gated<kAct>(a[i], b[i], limit, rate);
+        for (int i = 0; i < 8; ++i) {
+          v[i] = gated<kAct>(a[2 * i], a[2 * i + 1], limit, rate);
+          v[i + 8] = gated<kAct>(b[2 * i], b[2 * i + 1], limit, rate);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = gated<kAct>(a[i], b[i], limit, rate);
+      }
     }
     const float m = block_max(finite_max(v, kAmaxFloor));
-    const uint4 q = encode16(v, __fdiv_rn(kFp8Max, m));
+    uint4 q = encode16(v, __fdiv_rn(kFp8Max, m));
+    if (!kWideIn && wide_out) {   // (all lanes: a full block among the warp's is reason enough)
+      const uint4 packed = gather_codes(q);
+      if (left >= kScaleBlock) q = packed;
+    }
+    const bool packed_out = wide_out && left >= kScaleBlock;
     const float scale = __fdiv_rn(m, kFp8Max);
     auto put = [&](int r) {
       if (static_cast<unsigned>(r) >= static_cast<unsigned>(out_rows)) return;
-      write16(codes + static_cast<size_t>(static_cast<unsigned>(r)) * ld_codes + c0, n, wide_out, q);
+      uint8_t *dst = codes + static_cast<size_t>(static_cast<unsigned>(r)) * ld_codes;
+      if (packed_out) *reinterpret_cast<uint4 *>(dst + kb * kScaleBlock + lane * kQuantCols) = q;
+      else write_spread(dst + c0, n, q);
       if (lane == 0) scales[static_cast<size_t>(static_cast<unsigned>(r)) * ld_scales + kb] = scale;
     };
 #pragma unroll
@@ -167,16 +203,17 @@ quantize_fp8_kernel(const T *x, unsigned ld_x, int rows, int cols, unsigned n_bl
   }
 }
 
-// A CTA per 128 x 128 block: lane group g takes rows g, g + 32, ... of it.  2880 x 5760 x 32 bf16 weights: see the numbers of the
-// design notes' table; HBM-bound.
+// A CTA per 128 x 128 block: lane group g takes rows g, g + 32, ... of it.  Bound by HBM.
 template <class T>
 __global__ void __launch_bounds__(kQuantThreads)
-quantize_fp8_blocks_kernel(const T *w, size_t ld_w, int rows, int cols, uint8_t *codes, size_t ld_codes, float *scales, int wide_in, int wide_out) {
+quantize_fp8_blocks_kernel(const T *w, size_t ld_w, int rows, int cols, uint8_t *codes, size_t ld_codes, float *scales, int wide) {
   __shared__ float s_max[kQuantThreads / 32];
   grid_dep_sync();
   constexpr int kRows = kScaleBlock / kQuantGroups;   // of a thread
   const int lane = threadIdx.x % kQuantLanes, group = threadIdx.x / kQuantLanes;
-  const int r0 = blockIdx.y * kScaleBlock, c0 = blockIdx.x * kScaleBlock + lane * kQuantCols, n = cols - c0;
+  const int r0 = blockIdx.y * kScaleBlock;
+  const bool whole = wide && cols - static_cast<int>(blockIdx.x * kScaleBlock) >= kScaleBlock;   // (quantize_fp8_kernel)
+  const int c0 = blockIdx.x * kScaleBlock + lane * (whole ? kQuantCols : 1), n = cols - c0;
   const size_t mat = blockIdx.z;
   const T *src = w + mat * rows * ld_w;
   Raw16<T> raw[kRows];
@@ -184,7 +221,9 @@ quantize_fp8_blocks_kernel(const T *w, size_t ld_w, int rows, int cols, uint8_t 
 #pragma unroll
   for (int j = 0; j < kRows; ++j) {
     const int r = r0 + group + kQuantGroups * j;
-    raw[j].load(src + static_cast<size_t>(min(r, rows - 1)) * ld_w + c0, r < rows ? n : 0, wide_in);
+    const T *from = src + static_cast<size_t>(min(r, rows - 1)) * ld_w + c0;   // (a row again, where there is none: no other maximum)
+    if (whole) raw[j].load(from);
+    else raw[j].load_spread(from, n, kQuantLanes);
   }
   float v[16];
 #pragma unroll
@@ -205,7 +244,10 @@ quantize_fp8_blocks_kernel(const T *w, size_t ld_w, int rows, int cols, uint8_t 
     const int r = r0 + group + kQuantGroups * j;
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = raw[j][i];
-    if (r < rows) write16(codes + (mat * rows + r) * ld_codes + c0, n, wide_out, encode16(v, inv));
+    if (r >= rows) continue;
+    uint8_t *dst = codes + (mat * rows + r) * ld_codes + c0;
+    if (whole) *reinterpret_cast<uint4 *>(dst) = encode16(v, inv);
+    else write_spread(dst, n, encode16(v, inv));
   }
   if (threadIdx.x == 0) scales[(mat * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x] = __fdiv_rn(m, kFp8Max);
 }
@@ -245,13 +287,17 @@ int moe_quantize_fp8(moe_handle c, const void *x_dev, int dtype, long long ld_x,
     using T = decltype(type);
     return launch_kernel(kernel, dim3(grid), kQuantThreads, 0, static_cast<cudaStream_t>(stream), true, 0, static_cast<const T *>(x_dev),
                          static_cast<unsigned>(ld_x), rows, cols, static_cast<unsigned>(n_blocks), limit, rate, pair_row_dev, static_cast<unsigned>(fanout),
-                         out_rows, n_rows_dev, codes_dev, static_cast<unsigned>(ld_codes), scales_dev, static_cast<unsigned>(ld_scales), wide_in, wide_out);
+                         out_rows, n_rows_dev, codes_dev, static_cast<unsigned>(ld_codes), scales_dev, static_cast<unsigned>(ld_scales), wide_out);
   };
   auto by_act = [&](auto type) {
     using T = decltype(type);
-    return act == MOE_ACT_NONE     ? go(type, quantize_fp8_kernel<T, MOE_ACT_NONE>)
-           : act == MOE_ACT_SWIGLU ? go(type, quantize_fp8_kernel<T, MOE_ACT_SWIGLU>)
-                                   : go(type, quantize_fp8_kernel<T, MOE_ACT_SILU_MUL>);
+    auto by_alignment = [&](auto wide) {
+      constexpr bool kWide = decltype(wide)::value;
+      return act == MOE_ACT_NONE     ? go(type, quantize_fp8_kernel<T, MOE_ACT_NONE, kWide>)
+             : act == MOE_ACT_SWIGLU ? go(type, quantize_fp8_kernel<T, MOE_ACT_SWIGLU, kWide>)
+                                     : go(type, quantize_fp8_kernel<T, MOE_ACT_SILU_MUL, kWide>);
+    };
+    return wide_in ? by_alignment(std::true_type()) : by_alignment(std::false_type());
   };
   return launched(c, "moe_quantize_fp8", dtype == MOE_F32 ? by_act(float()) : dtype == MOE_BF16 ? by_act(__nv_bfloat16()) : by_act(__half()));
 }
@@ -271,7 +317,7 @@ int moe_quantize_fp8_blocks(moe_handle c, const void *w_dev, int dtype, long lon
   auto go = [&](auto type) {
     using T = decltype(type);
     return launch_kernel(quantize_fp8_blocks_kernel<T>, grid, kQuantThreads, 0, static_cast<cudaStream_t>(stream), true, 0, static_cast<const T *>(w_dev),
-                         static_cast<size_t>(ld_w), rows, cols, codes_dev, static_cast<size_t>(ld_codes), scales_dev, wide_in, wide_out);
+                         static_cast<size_t>(ld_w), rows, cols, codes_dev, static_cast<size_t>(ld_codes), scales_dev, wide_in && wide_out);
   };
   return launched(c, "moe_quantize_fp8_blocks", dtype == MOE_F32 ? go(float()) : dtype == MOE_BF16 ? go(__nv_bfloat16()) : go(__half()));
 }

@@ -13,11 +13,13 @@ namespace moe {
 // lower index;  weight = s [/ sum of the selected s] * scale.  An expert is off where x or its bias is -inf or NaN.
 //
 // Which of two neighbouring p is larger is part of the answer, so the comparisons are those of 64 bits.  A row is tried in
-// 32 bits first.  There a sigmoid is off by less than 2^-21 (s (1 - s) times the exponential's (2 + 1.2 |x|) 2^-23, and the
-// roundings of sum and quotient), a softmax by less than 2^-18 of the row's largest (exponentials, a sum of up to 512, a quotient);
-// so an order is certain where two values differ by 2^-20, or 2^-17 of that largest, and 2^-22 of their own magnitudes (twice
-// that for sums of two).  A row with a closer call (equal scores, scores that saturate) is done again in 64 bits: 4 us more for a
-// call of 8192 rows in which one row in a hundred is, however few.
+// 32 bits first.  Without a bias the scores are in the order of the logits, and these are compared; only where 64 bits themselves
+// no longer tell scores apart (a sigmoid above 16, logits within 1e-9) is the order not theirs.  With a bias a sigmoid in 32 bits
+// is off by less than 2^-21 (s (1 - s) times the exponential's (2 + 1.2 |x|) 2^-23, and the roundings of sum and quotient), a
+// softmax by less than 2^-18 of the row's largest (exponentials, a sum of up to 512, a quotient); so an order is certain where two
+// values differ by 2^-20, or 2^-17 of that largest, and 2^-22 of their own magnitudes (twice that for sums of two), or where
+// both logits and both biases are equal: then the index decides.  A row with a closer call is done again in 64 bits, in
+// code that is cold: 3 us more for a call of 8192 rows, however few they are.
 //
 // A warp per row; lane l owns the per_lane consecutive experts from l * per_lane, so that a lower lane is a lower index.
 // ---------------------------------------------------------------------------
@@ -57,69 +59,193 @@ __device__ __forceinline__ R warp_sum(R v) {
   return v;
 }
 
-// One row with scores of type R.  x[i]: the lane's logits, -inf where there is none.  Lane k < top_k receives the k-th selected
-// expert (or -1) in `sel`.  R = float: returns false where 32 bits do not settle a comparison.  `top` and `sum`: of the softmax.
-// `group_lanes`: lanes of a group, where groups are runs of whole lanes, a power of two of them; else 0 and `shared` is used.
-template <class R, int kPer>
-__device__ __forceinline__ bool select_experts(const float (&x)[kPer], const float (&b)[kPer], const moe_route_rule &rule, int per_lane, int group_lanes,
-                                               unsigned long long *shared, int lane, float top, double &sum, int &sel, R &sel_s) {
-  constexpr bool kFast = sizeof(R) == 4;
-  using Key = decltype(ordered_key(R()));
+// The two largest keys of every group, in all of its lanes: a group is `lanes` whole lanes, a power of two.
+template <class Key, int kPer>
+__device__ __forceinline__ void two_best(const Key (&key)[kPer], int lanes, Key &k1, Key &k2) {
+  k1 = k2 = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    k2 = max(k2, min(k1, key[i]));
+    k1 = max(k1, key[i]);
+  }
+  for (int off = 1; off < lanes; off <<= 1) {
+    const Key o1 = __shfl_xor_sync(0xffffffffu, k1, off), o2 = __shfl_xor_sync(0xffffffffu, k2, off);
+    k2 = max(max(k2, o2), min(k1, o1));
+    k1 = max(k1, o1);
+  }
+}
+// Lane g < n_groups holds what group g is worth: its rank, equal ones by the lower index.
+template <class Key>
+__device__ __forceinline__ int group_rank(Key worth, int n_groups, int lane) {
+  int better = 0;
+  for (int g = 0; g < n_groups; ++g) {
+    const Key k = __shfl_sync(0xffffffffu, worth, g);
+    better += k > worth || (k == worth && g < lane);
+  }
+  return lane < n_groups ? better : 32;
+}
+// One round of the selection: the largest key left in the warp, of the lowest lane that has it, and in that lane the lowest expert.
+// Returns the key (0: nothing left); the owner's key is taken out.
+template <class Key, int kPer>
+__device__ __forceinline__ Key take_best(Key (&key)[kPer], Key &best, int lane, int &at, int &owner) {
+  unsigned owners;
+  const Key top = warp_best(best, owners);
+  if (top == 0) return 0;
+  owner = __ffs(owners) - 1;
+  at = 0;
+  if (lane == owner) {
+    Key next = 0;
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const bool hit = !found && key[i] == top;
+      if (hit) {
+        at = i;
+        key[i] = 0;
+      }
+      found = found || hit;
+      next = max(next, key[i]);
+    }
+    best = next;
+  }
+  at = __shfl_sync(0xffffffffu, at, owner);
+  return top;
+}
+
+// One row in 32 bits.  x[i]: the lane's logits, -inf where there is none; b[i]: its biases, -inf where there is no expert.  Lane
+// k < top_k receives the k-th selected expert (or -1) in `sel`.  `top` and `sum`: of the softmax.  Returns false where 32 bits do
+// not settle a comparison.  Groups are `group_lanes` whole lanes.
+template <class T, int kPer>
+__device__ __forceinline__ bool select_fast(const T *src, const float (&x)[kPer], const float *bias, const float (&b)[kPer], const moe_route_rule &rule,
+                                            int per_lane, int group_lanes, int lane, float top, float &sum, int &sel) {
   const float inf = __int_as_float(0x7f800000);
-  const int first = lane * per_lane;
-  R s[kPer];
-  Key key[kPer];
-  R bound = 1;   // no s is larger
-  if (rule.score == MOE_SCORE_SOFTMAX) {
-    R part = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      if constexpr (kFast) s[i] = x[i] > -inf ? __expf(x[i] - top) : 0.f;
-      else s[i] = x[i] > -inf ? exp(static_cast<double>(x[i]) - static_cast<double>(top)) : 0.0;
-      part += s[i];
-    }
-    part = warp_sum(part);
-    sum = part;
-    bound = part > 0 ? R(1) / part : R(0);
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      if constexpr (kFast) s[i] *= bound;
-      else if (part > 0) s[i] /= part;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      if constexpr (kFast) s[i] = __fdividef(1.f, 1.f + __expf(-x[i]));
-      else s[i] = 1.0 / (1.0 + exp(-static_cast<double>(x[i])));
-    }
-  }
-  const R close = rule.score == MOE_SCORE_SOFTMAX ? bound * R(7.62939453125e-06) : R(9.5367431640625e-07);   // 2^-17, 2^-20
-  const R rel = R(2.384185791015625e-07);   // 2^-22
-  auto certain = [&](Key a, Key b, R twice) {   // a is the larger of two keys that are on
-    const R va = key_value(a), vb = key_value(b);
-    return va - vb > twice * (close + rel * (fabs(va) + fabs(vb)));
-  };
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {   // (b: -inf where the lane has no expert)
-    key[i] = ordered_key(s[i] + static_cast<R>(b[i]));
-    if (!(x[i] > -inf) || !(b[i] > -inf)) key[i] = 0;
-  }
-  bool settled = true;
-  if (rule.n_groups > 1) {
-    // lane g < n_groups: what group g is worth, from its two largest
-    const int size = rule.n_experts / rule.n_groups;
-    Key k1 = 0, k2 = 0;
-    if (kFast || group_lanes > 0) {
+  const bool softmax = rule.score == MOE_SCORE_SOFTMAX;
+  auto score = [&](float v) { return softmax ? __expf(v - top) : __fdividef(1.f, 1.f + __expf(-v)); };
+  float over = 1.f;   // a softmax is score * over
+  unsigned key[kPer];
+  if (bias != nullptr || (softmax && !rule.renormalise)) {
+    float s[kPer];
+    if (softmax) {
+      sum = 0.f;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        k2 = max(k2, min(k1, key[i]));
-        k1 = max(k1, key[i]);
+        s[i] = x[i] > -inf ? __expf(x[i] - top) : 0.f;
+        sum += s[i];
       }
-      for (int off = 1; off < group_lanes; off <<= 1) {
-        const Key o1 = __shfl_xor_sync(0xffffffffu, k1, off), o2 = __shfl_xor_sync(0xffffffffu, k2, off);
-        k2 = max(max(k2, o2), min(k1, o1));
-        k1 = max(k1, o1);
+      sum = warp_sum(sum);
+      over = sum > 0.f ? __fdividef(1.f, sum) : 0.f;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) s[i] = __fdividef(1.f, 1.f + __expf(-x[i]));
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) key[i] = bias != nullptr ? ordered_key(fmaf(s[i], over, b[i])) : ordered_key(x[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) key[i] = ordered_key(x[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < kPer; ++i)
+    if (!(x[i] > -inf) || !(b[i] > -inf)) key[i] = 0;
+  const float close = softmax ? over * 7.62939453125e-06f : 9.5367431640625e-07f, rel = 2.384185791015625e-07f;   // 2^-17, 2^-20, 2^-22
+  auto far_apart = [&](float a, float c, float twice) { return a - c > twice * (close + rel * (fabsf(a) + fabsf(c))); };
+  // the order of two keys (the first is not the smaller) is that of 64 bits
+  auto certain = [&](unsigned ka, unsigned kc) {
+    const float a = key_value(ka), c = key_value(kc);
+    if (bias != nullptr) return far_apart(a, c, 1.f);
+    const bool resolved = softmax ? c > top - 600.f : a < 16.f && c > -600.f;
+    return resolved && (ka == kc || a - c > 1e-9f);
+  };
+  bool settled = true;
+  if (rule.n_groups > 1) {
+    unsigned k1, k2;
+    two_best(key, group_lanes, k1, k2);
+    k1 = __shfl_sync(0xffffffffu, k1, lane * group_lanes & 31);   // lane g: those of group g
+    k2 = __shfl_sync(0xffffffffu, k2, lane * group_lanes & 31);
+    if (lane >= rule.n_groups) k1 = k2 = 0;
+    unsigned worth = k1;
+    const bool sums = rule.group_top == 2;
+    if (sums && k1 != 0) {
+      auto value = [&](unsigned k) { return k == 0 ? 0.f : bias != nullptr ? key_value(k) : score(key_value(k)) * over; };
+      worth = ordered_key(value(k1) + value(k2));
+    }
+    const int rank = group_rank(worth, rule.n_groups, lane);
+    const unsigned stays = __ballot_sync(0xffffffffu, rank < rule.top_groups);
+    if (rule.top_groups < rule.n_groups) {   // the last group that stays against the first that does not
+      const int in = __ffs(__ballot_sync(0xffffffffu, rank == rule.top_groups - 1)) - 1, out = __ffs(__ballot_sync(0xffffffffu, rank == rule.top_groups)) - 1;
+      const unsigned a1 = __shfl_sync(0xffffffffu, k1, in), a2 = __shfl_sync(0xffffffffu, k2, in), wa = __shfl_sync(0xffffffffu, worth, in);
+      const unsigned c1 = __shfl_sync(0xffffffffu, k1, out), c2 = __shfl_sync(0xffffffffu, k2, out), wc = __shfl_sync(0xffffffffu, worth, out);
+      if (wc != 0) {
+        if (!sums) settled = certain(a1, c1);
+        else if (bias == nullptr && a1 == c1 && a2 == c2) settled = true;
+        else settled = far_apart(key_value(wa), key_value(wc), 2.f);
       }
+    }
+    if (!(stays >> (lane / group_lanes) & 1u)) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) key[i] = 0;
+    }
+  }
+  // one round more than experts, for the first that is not selected: lane k keeps the k-th, and neighbours are compared at the end
+  sel = -1;
+  unsigned best = key[0], kept = 0, beyond = 0;
+#pragma unroll
+  for (int i = 1; i < kPer; ++i) best = max(best, key[i]);
+  int next_sel = -1;   // of lane 31: the expert of round 32
+  for (int k = 0; k <= rule.top_k; ++k) {
+    int at, owner;
+    const unsigned top_key = take_best(key, best, lane, at, owner);
+    if (top_key == 0) break;
+    const int e = owner * per_lane + at;
+    if (lane == k) { kept = top_key; sel = e; }
+    if (k == 32) { beyond = top_key; next_sel = e; }
+  }
+  unsigned after = __shfl_down_sync(0xffffffffu, kept, 1);
+  int after_sel = __shfl_down_sync(0xffffffffu, sel, 1);
+  if (lane == 31) { after = beyond; after_sel = next_sel; }
+  if (lane < rule.top_k && kept != 0 && after != 0 && !certain(kept, after)) {
+    // equal logits under equal biases: the index has decided
+    const bool same = bias != nullptr && to_f32(src[sel]) == to_f32(src[after_sel]) && bias[sel] == bias[after_sel];
+    if (!same) settled = false;
+  }
+  if (lane >= rule.top_k) sel = -1;
+  return __all_sync(0xffffffffu, settled);
+}
+
+// One row in 64 bits; sel_s: the score of the selected.  With group_lanes = 0 groups are any runs of experts, through `shared`.
+template <int kPer>
+__device__ __forceinline__ void select_exact(const float (&x)[kPer], const float (&b)[kPer], const moe_route_rule &rule, int per_lane, int group_lanes,
+                                             unsigned long long *shared, int lane, float top, int &sel, double &sel_s) {
+  using Key = unsigned long long;
+  const float inf = __int_as_float(0x7f800000);
+  const int first = lane * per_lane;
+  double s[kPer];
+  Key key[kPer];
+  if (rule.score == MOE_SCORE_SOFTMAX) {
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      s[i] = x[i] > -inf ? exp(static_cast<double>(x[i]) - static_cast<double>(top)) : 0.0;
+      sum += s[i];
+    }
+    sum = warp_sum(sum);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (sum > 0.0) s[i] /= sum;
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) s[i] = 1.0 / (1.0 + exp(-static_cast<double>(x[i])));
+  }
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    key[i] = ordered_key(s[i] + static_cast<double>(b[i]));
+    if (!(x[i] > -inf) || !(b[i] > -inf)) key[i] = 0;
+  }
+  if (rule.n_groups > 1) {
+    const int size = rule.n_experts / rule.n_groups;
+    Key k1 = 0, k2 = 0;
+    if (group_lanes > 0) {
+      two_best(key, group_lanes, k1, k2);
     } else {
 #pragma unroll
       for (int i = 0; i < kPer; ++i)
@@ -127,7 +253,7 @@ __device__ __forceinline__ bool select_experts(const float (&x)[kPer], const flo
       __syncwarp();
       if (lane < rule.n_groups)
         for (int j = 0; j < size; ++j) {
-          const Key k = static_cast<Key>(shared[lane * size + j]);
+          const Key k = shared[lane * size + j];
           k2 = max(k2, min(k1, k));
           k1 = max(k1, k);
         }
@@ -136,75 +262,29 @@ __device__ __forceinline__ bool select_experts(const float (&x)[kPer], const flo
     if (rule.group_top == 2 && k2) worth = ordered_key(key_value(k1) + key_value(k2));
     if (group_lanes > 0) worth = __shfl_sync(0xffffffffu, worth, lane * group_lanes & 31);
     if (lane >= rule.n_groups) worth = 0;
-    int better = 0;
-    for (int g = 0; g < rule.n_groups; ++g) {
-      const Key k = __shfl_sync(0xffffffffu, worth, g);
-      better += k > worth || (k == worth && g < lane);
-    }
-    const unsigned stays = __ballot_sync(0xffffffffu, lane < rule.n_groups && better < rule.top_groups);
-    if (kFast && rule.top_groups < rule.n_groups) {   // the last group that stays against the first that does not
-      const unsigned in = __ballot_sync(0xffffffffu, lane < rule.n_groups && better == rule.top_groups - 1);
-      const unsigned out = __ballot_sync(0xffffffffu, lane < rule.n_groups && better == rule.top_groups);
-      const Key a = __shfl_sync(0xffffffffu, worth, __ffs(in) - 1), b = __shfl_sync(0xffffffffu, worth, __ffs(out) - 1);
-      if (b != 0 && !certain(a, b, R(2))) settled = false;
-    }
-    if (kFast || group_lanes > 0) {
-      if (!(stays >> (lane / group_lanes) & 1u)) {
+    const unsigned stays = __ballot_sync(0xffffffffu, group_rank(worth, rule.n_groups, lane) < rule.top_groups);
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) key[i] = 0;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (i < per_lane && first + i < rule.n_experts && !(stays >> ((first + i) / size) & 1u)) key[i] = 0;
-    }
+    for (int i = 0; i < kPer; ++i)
+      if (i < per_lane && first + i < rule.n_experts && !(stays >> ((first + i) / size) & 1u)) key[i] = 0;
   }
-  // rounds: the largest key of a lane, then of the warp; the lowest lane of equal ones, and in it the lowest expert.  In 32 bits
-  // one round more, for the first that is not selected: lane k keeps the k-th key, and neighbours are compared at the end.
   sel = -1;
-  sel_s = 0;
-  Key best = key[0], kept = 0;
+  sel_s = 0.0;
+  Key best = key[0];
 #pragma unroll
   for (int i = 1; i < kPer; ++i) best = max(best, key[i]);
-  const int rounds = rule.top_k + (kFast ? 1 : 0);
-  Key beyond = 0;   // of the round that has no lane
-  for (int k = 0; k < rounds; ++k) {
-    unsigned owners;
-    const Key top_key = warp_best(best, owners);
-    if (top_key == 0) break;   // nothing left
-    if (lane == k) kept = top_key;
-    if (k == 32) beyond = top_key;
-    if (kFast && k == rule.top_k) break;
-    const int owner = __ffs(owners) - 1;
-    int e = 0;
-    R es = 0;
-    if (lane == owner) {
-      Key next = 0;
-      bool found = false;
+  for (int k = 0; k < rule.top_k; ++k) {
+    int at, owner;
+    if (take_best(key, best, lane, at, owner) == 0) break;
+    double mine = 0.0;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const bool hit = !found && key[i] == top_key;
-        if (hit) {
-          e = first + i;
-          if (!kFast) es = s[i];
-          key[i] = 0;
-        }
-        found = found || hit;
-        next = max(next, key[i]);
-      }
-      best = next;
+    for (int i = 0; i < kPer; ++i)
+      if (i == at) mine = s[i];
+    mine = __shfl_sync(0xffffffffu, mine, owner);
+    if (lane == k) {
+      sel = owner * per_lane + at;
+      sel_s = mine;
     }
-    e = __shfl_sync(0xffffffffu, e, owner);
-    if (!kFast) es = __shfl_sync(0xffffffffu, es, owner);
-    if (lane == k) { sel = e; sel_s = es; }
   }
-  if (kFast) {
-    Key after = __shfl_down_sync(0xffffffffu, kept, 1);
-    if (lane == 31) after = beyond;
-    const bool close_call = lane < rule.top_k && kept != 0 && after != 0 && !certain(kept, after, R(1));
-    if (__any_sync(0xffffffffu, close_call)) settled = false;
-  }
-  return settled;
 }
 
 template <class T, int kPer>
@@ -267,10 +347,9 @@ route_scored_kernel(const T *logits, size_t ld, const float *bias, int rows, moe
     if (!(top > -inf)) top = 0.f;
   }
   int sel;
-  double sum = 0.0, share = 0.0;
-  float unused;
-  if ((rule.n_groups == 1 || group_lanes > 0) &&
-      select_experts<float, kPer>(x, b, rule, per_lane, group_lanes, nullptr, lane, top, sum, sel, unused)) {
+  double share = 0.0;
+  float sum = 0.f;
+  if ((rule.n_groups == 1 || group_lanes > 0) && select_fast(src, x, bias, b, rule, per_lane, group_lanes, lane, top, sum, sel)) {
     // weights of the selected from their logits, within a few roundings of 32 bits
     float s = 0.f;
     if (sel >= 0) {
@@ -288,11 +367,11 @@ route_scored_kernel(const T *logits, size_t ld, const float *bias, int rows, moe
       const float all = warp_sum(s);
       share = all > 0.f ? __fdiv_rn(s, all) : 0.f;
     } else {
-      share = rule.score == MOE_SCORE_SOFTMAX && sum > 0.0 ? s / sum : s;
+      share = rule.score != MOE_SCORE_SOFTMAX ? s : sum > 0.f ? __fdiv_rn(s, sum) : 0.f;
     }
   } else {
     double s;
-    select_experts<double, kPer>(x, b, rule, per_lane, group_lanes, s_keys[warp], lane, top, sum, sel, s);
+    select_exact(x, b, rule, per_lane, group_lanes, s_keys[warp], lane, top, sel, s);
     share = s;
     if (rule.renormalise) {
       const double all = warp_sum(s);

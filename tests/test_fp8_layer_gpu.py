@@ -64,6 +64,8 @@ def check_route(got, want):
 
 
 @pytest.mark.parametrize("rows,experts,top_k,groups,top_groups,group_top,score,dtype,bias,pad", [
+    (40, 510, 8, 2, 1, 2, "sigmoid", "f32", True, 0),      # groups that are not whole lanes
+    (40, 496, 6, 16, 5, 2, "softmax", "bf16", False, 0),
     (1, 128, 4, 1, 1, 1, "softmax", "f32", False, 0),
     (1, 256, 8, 8, 4, 2, "sigmoid", "f32", True, 0),
     (5, 1, 1, 1, 1, 1, "sigmoid", "f32", True, 0),
@@ -124,6 +126,19 @@ def test_route_next_to_a_tie_is_decided_in_64_bits(pkg, handle):
     for score in ("sigmoid", "softmax"):
         args = dict(top_k=6, score=score)
         check_route(run_route(pkg, handle, x, b, **args), ref.route(x, b, **args))
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("groups,group_top", [(1, 1), (8, 1), (8, 2)])
+@pytest.mark.parametrize("bias", ["none", "zero", "steps"])
+def test_route_many_equal_scores(score, groups, group_top, bias, pkg, handle):
+    """Logits of a coarse grid: equal scores, equal groups and, under a bias of the same grid, equal sums of different parts."""
+    g = gen(11)
+    x = (randn(g, 400, 64) * 4).round() / 4
+    x[300:] *= 12                                     # sigmoids that 64 bits no longer tell apart
+    b = None if bias == "none" else torch.zeros(64, device="cuda") if bias == "zero" else (randn(g, 64) * 4).round() / 16
+    args = dict(top_k=8, score=score, n_groups=groups, top_groups=max(1, groups // 2), group_top=group_top)
+    check_route(run_route(pkg, handle, x.bfloat16(), b, dtype="bf16", **args), ref.route(x.bfloat16(), b, **args))
 
 
 def test_route_agrees_with_the_softmax_rule_of_the_block(pkg):
@@ -346,9 +361,9 @@ def test_dense_product(rows, n, k, out, bias, pkg, handle):
     check_product(p, run_product(pkg, handle, p, out), out)
 
 
-@pytest.mark.parametrize("pad", [0, 1, 8])
+@pytest.mark.parametrize("pad", [0, 1, 2, 8])
 @pytest.mark.parametrize("out", ["f16", "bf16", "f32"])
-@pytest.mark.parametrize("rows", [5, 200])
+@pytest.mark.parametrize("rows", [5, 40, 100, 200, 9000])
 def test_product_output_types_and_strides(rows, out, pad, pkg, handle):
     p = make_product(pad, rows, 264, 400, bias=True)
     p["sa"] *= 0.01          # inside the range of fp16
