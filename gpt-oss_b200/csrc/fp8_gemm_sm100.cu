@@ -7,11 +7,28 @@
 // tensor memory; the outer one, with its two scales, is one multiply-add per element and block on the CUDA cores, in fp32
 // registers.
 //
-// The weights are the M operand: a tile is one row of scale blocks (128 weight rows, a lane of tensor memory each) against up
-// to kTok token rows on N, which follows the number of rows of the group in steps of 16.  sb is then one number per tile and
-// block, and sa * sb a vector over the columns of the accumulator that a warp of its own forms in shared memory.  The
-// accumulators are read as fragments (a thread has two neighbouring columns of four rows): an 8-byte load of scales then serves
-// four packed multiply-adds, where a row per thread would load every scale of the tile in every thread.
+// That outer sum is what these kernels are shaped by.  The codes of a block of k go from HBM through TMA to the tensor core
+// untouched, but every fp32 partial product comes back through registers once per 128 of k.
+//
+// Few rows per group (fp8_gemm_kernel).  The weights are the M operand: a tile is one row of scale blocks (128 weight rows, a lane of
+// tensor memory each) against up to kTok token rows on N, which follows the number of rows of the group in steps of 16.  sb is
+// then one number per tile and block, and sa * sb a vector over the columns of the accumulator that a warp of its own forms in
+// shared memory.  The accumulators are read as fragments (a thread has two neighbouring columns of four rows): an 8-byte load of
+// scales then serves four packed multiply-adds.  With a row per thread every scale of the tile is loaded in every thread, and a
+// block of 128 x 128 took 700 cycles for its multiply-adds instead of 120, although the tensor-memory loads of fragments are
+// slower (128 cycles of a quadrant for 64 columns, 35 for rows).  Bound by HBM: 256 rows over 32 experts of 5760 x 2880 85 us =
+// 6.3 TB/s.  One decode step (16 x 4096 x 7168) 8.7 us for the 4.5 that its weights take: launch, 14 blocks of k, and the sum
+// of four CTAs' parts.
+//
+// Many rows per group (fp8_gemm_wide_kernel).  128 token rows x 256 weight rows; the token rows are the M operand, so that sa * sb
+// is one number per thread and block.  8192 x 4096 x 7168 224 us = 2.1 PFLOP/s, 6144 rows over 32 experts of 5760 x 2880 175 us,
+// both at the power cap: the clock falls to 1.36 GHz.  In cycles a block of k takes 775 (dense) for 512 of tensor pipe; two
+// accumulators of 256 columns are all that tensor memory holds, and one comes back for its next block after the MMA (512), the
+// wait that sees it done (180), eight loads of 16 columns with their multiply-adds (600) and the wait of the MMA warp (150).
+// Measured and set aside: pairs of CTAs (cta_group::2, 256 x 256), which move a third less through shared memory, 226 us for the
+// experts (tiles of 256 rows waste 62 % on groups of 192, those of 128 32 %) and 260 for the dense case; halves of 128 columns
+// with an MMA warp each, the same; the next barrier looked up ahead of time, 4 to 8 % slower; loads of 32 columns in two
+// buffers, slower by what spills (the accumulators are 128 registers of 168).
 #include <cuda_fp8.h>
 
 #include "fp8_layer.cuh"
@@ -41,14 +58,14 @@ constexpr int kWeightTile = kScaleBlock * kScaleBlock;   // bytes of a tile's we
 
 template <int kTok>
 struct GemmShape {
-  static constexpr int kBoxRows = kTok <= 32 ? 16 : kTok / 2;     // token rows of a copy
+  static_assert(kTok == 16 || kTok == 64 || kTok == 128, "the forms of gemm_form");
+  static constexpr int kBoxRows = kTok == 16 ? 16 : kTok / 2;     // token rows of a copy
   static constexpr int kStageBytes = kWeightTile + kTok * kScaleBlock;
-  static constexpr int kEpiWarps = kTok <= 64 ? 4 : kTok / 16;
+  static constexpr int kEpiWarps = kTok <= 64 ? 4 : 8;
   static constexpr int kCols = kTok / (kEpiWarps / 4);            // accumulator columns of a warp
-  static constexpr int kChunk = kCols < 32 ? kCols : kTok > 128 ? 32 : kCols;   // of these, fetched from tensor memory at once
   static constexpr int kBufCols = kTok < 32 ? 32 : kTok;
-  static constexpr int kAccBufs = kTok > 128 ? 2 : 4;             // accumulators: blocks of k under way
-  static constexpr int kTmemCols = kTok > 128 ? 512 : kAccBufs * kBufCols;   // a power of two
+  static constexpr int kAccBufs = 4;                              // accumulators: blocks of k under way
+  static constexpr int kTmemCols = kAccBufs * kBufCols;
   static constexpr int kThreads = (kEpiWarps + 3) * 32;           // + copies, MMA, scales
   static constexpr int kPartPitch = kScaleBlock + 4;              // floats of a token's partial sums: no bank conflicts
   static constexpr int kOutPitch = 80;                            // bytes of 32 16-bit outputs of a token, the same
@@ -149,7 +166,7 @@ __device__ __forceinline__ void add_up_splits(const Fp8GemmArgs &p, const GemmTi
   }
 }
 
-// Offsets that are not ascending give wrong rows, never rows outside.
+// Offsets that are not ascending give wrong rows or none, never rows outside.
 __device__ __forceinline__ int group_begin(const Fp8GemmArgs &p, int g) { return p.offsets == nullptr ? 0 : min(max(p.offsets[g], 0), p.rows); }
 __device__ __forceinline__ int group_end(const Fp8GemmArgs &p, int g) { return p.offsets == nullptr ? p.rows : min(max(p.offsets[g + 1], 0), p.rows); }
 
@@ -170,12 +187,20 @@ __device__ __forceinline__ void count_tiles(const Fp8GemmArgs &p, int *s_tiles) 
       if (g0 + lane < p.n_groups) s_tiles[g0 + lane + 1] = before + v;
       before += __shfl_sync(0xffffffffu, v, 31);
     }
-    if (lane == 0) s_tiles[0] = 0;
+    if (lane == 0) {
+      s_tiles[0] = 0;
+      // ascending offsets cannot give more (and what the host sized the grid for stays true)
+      if (before < 0 || before > p.rows / kTok + p.n_groups) s_tiles[p.n_groups] = 0;
+    }
   }
   __syncthreads();
 }
-// Item -> tile, of n_nb weight blocks per group: the token tiles of a weight block follow one another.  The tiles of a group
-// are of equal size in steps of 16 rows; none is empty.
+// Item -> tile, of n_nb weight blocks per group: the token tiles of a weight block follow one another, in runs of kRunTiles of a
+// group's tiles.  So the CTAs that are at work share a dozen token tiles and a dozen weight blocks: with all tiles of a group in
+// one run 65536 x 4096 x 4096 took 1465 us (token rows again from HBM for every weight block), with 8 / 12 / 16 / 32 of them
+// 1170 / 1140 / 1180 / 1170, 8192 x 4096 x 7168 233 and 226 / 224 / 227 / 226.  The tiles of a group are of equal size in steps of
+// 16 rows; none is empty.
+constexpr int kRunTiles = 12;
 __device__ __forceinline__ GemmTile tile_at(const Fp8GemmArgs &p, const int *s_tiles, int item, int n_nb) {
   const int q = item / n_nb;
   int lo = 0, hi = p.n_groups;   // s_tiles[lo] <= q < s_tiles[hi]
@@ -187,8 +212,9 @@ __device__ __forceinline__ GemmTile tile_at(const Fp8GemmArgs &p, const int *s_t
   const int local = item - s_tiles[lo] * n_nb;
   const int begin = group_begin(p, lo), cnt = group_end(p, lo) - begin;
   const int per = ((cnt + tiles - 1) / tiles + 15) / 16 * 16;
-  const int row = (local % tiles) * per;
-  return GemmTile{lo, local / tiles, begin + row, min(per, cnt - row)};
+  const int run = local / (kRunTiles * n_nb), in_run = local - run * kRunTiles * n_nb, width = min(kRunTiles, tiles - run * kRunTiles);
+  const int row = (run * kRunTiles + in_run % width) * per;
+  return GemmTile{lo, in_run / width, begin + row, min(per, cnt - row)};
 }
 
 template <int kTok>
@@ -291,7 +317,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
     }
   } else if (warp == kScaleWarp) {
     // ---- scales of the tile's tokens times the block's own, kScaleBlocks blocks of k to a slot
-    constexpr int kPer = kTok < 32 ? 1 : kTok / 32, kPass = kPer < 4 ? kPer : 4;   // tokens of a lane; of these, fetched together
+    constexpr int kPer = kTok < 32 ? 1 : kTok / 32;   // tokens of a lane
     uint32_t s = 0, par = 1u, plan = 0, ppar = 1u;
     float *slots = reinterpret_cast<float *>(ring_ptr + S::kScaleOff);
     for (int it = blockIdx.x; ok && it < n_items; it += stride) {
@@ -313,26 +339,22 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
       const float *sb = p.sb + (static_cast<size_t>(t.g) * n_nb + t.nb) * p.n_kb;
       for (int k0 = kb0; ok && k0 < kb1; k0 += kScaleBlocks) {
         const float b = lane < kScaleBlocks && k0 + lane < kb1 ? sb[k0 + lane] : 0.f;
+        float v[kPer][kScaleBlocks];
 #pragma unroll
-        for (int i0 = 0; i0 < kPer; i0 += kPass) {
-          float v[kPass][kScaleBlocks];
+        for (int i = 0; i < kPer; ++i) {
+          const int tok = lane + 32 * i;
+          const float *sa = p.sa + static_cast<size_t>(t.row0 + tok) * p.ld_sa + k0;
 #pragma unroll
-          for (int i = 0; i < kPass; ++i) {
-            const int tok = lane + 32 * (i0 + i);
-            const float *sa = p.sa + static_cast<size_t>(t.row0 + tok) * p.ld_sa + k0;
-#pragma unroll
-            for (int j = 0; j < kScaleBlocks; ++j) v[i][j] = tok < t.ntok && k0 + j < kb1 ? sa[j] : 0.f;
-          }
-          if (i0 == 0 && !mbar_wait_warp(sempty(s), par, abort_flag, p.status, ST_WAIT_AFREE)) { ok = false; break; }
-#pragma unroll
-          for (int j = 0; j < kScaleBlocks; ++j) {
-            const float f = __shfl_sync(0xffffffffu, b, j);
-#pragma unroll
-            for (int i = 0; i < kPass; ++i)
-              if (lane + 32 * (i0 + i) < kTok) slots[(s * kScaleBlocks + j) * kTok + lane + 32 * (i0 + i)] = v[i][j] * f;
-          }
+          for (int j = 0; j < kScaleBlocks; ++j) v[i][j] = tok < t.ntok && k0 + j < kb1 ? sa[j] : 0.f;
         }
-        if (!ok) break;
+        if (!mbar_wait_warp(sempty(s), par, abort_flag, p.status, ST_WAIT_AFREE)) { ok = false; break; }
+#pragma unroll
+        for (int j = 0; j < kScaleBlocks; ++j) {
+          const float f = __shfl_sync(0xffffffffu, b, j);
+#pragma unroll
+          for (int i = 0; i < kPer; ++i)
+            if (lane + 32 * i < kTok) slots[(s * kScaleBlocks + j) * kTok + lane + 32 * i] = v[i][j] * f;
+        }
         __syncwarp();
         if (lane == 0) mbar_arrive(sfull(s));
         if (++s == kScaleSlots) { s = 0; par ^= 1u; }
@@ -359,35 +381,30 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
         tc_fence_after();
         const uint32_t src = tmem + lane_field + d * S::kBufCols + col0;
         const float *f = slots + (s * kScaleBlocks + kq) * kTok;
+        constexpr int kLd = S::kCols < 32 ? 16 : 32;   // columns of a load
+        uint32_t v[S::kCols / kLd][2][kLd / 2];
 #pragma unroll
-        for (int c = 0; c < S::kCols; c += S::kChunk) {
-          constexpr int kLd = S::kChunk < 32 ? 16 : 32;   // columns of a load
-          uint32_t v[S::kChunk / kLd][2][kLd / 2];
-#pragma unroll
-          for (int l = 0; l < S::kChunk / kLd; ++l)
-            if (col0 + c + l * kLd < t.ntok) {
-              tmem_ld_frag(src + c + l * kLd, v[l][0]);
-              tmem_ld_frag(src + c + l * kLd + (16u << 16), v[l][1]);
-            }
-          tmem_wait_ld();
-          if (c + S::kChunk == S::kCols) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(dempty(d));
+        for (int l = 0; l < S::kCols / kLd; ++l)
+          if (col0 + l * kLd < t.ntok) {
+            tmem_ld_frag(src + l * kLd, v[l][0]);
+            tmem_ld_frag(src + l * kLd + (16u << 16), v[l][1]);
           }
+        tmem_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(dempty(d));
 #pragma unroll
-          for (int l = 0; l < S::kChunk / kLd; ++l)
-            if (col0 + c + l * kLd < t.ntok) {
+        for (int l = 0; l < S::kCols / kLd; ++l)
+          if (col0 + l * kLd < t.ntok) {
 #pragma unroll
-              for (int j = 0; j < kLd / 8; ++j) {
-                const uint64_t f2 = *reinterpret_cast<const uint64_t *>(f + c + l * kLd + 8 * j);
+            for (int j = 0; j < kLd / 8; ++j) {
+              const uint64_t f2 = *reinterpret_cast<const uint64_t *>(f + l * kLd + 8 * j);
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+              for (int h = 0; h < 2; ++h)
 #pragma unroll
-                  for (int i = 0; i < 2; ++i) fma_f32x2(acc[(c + l * kLd) / 8 + j][h][i], v[l][h][4 * j + 2 * i], v[l][h][4 * j + 2 * i + 1], f2);
-              }
+                for (int i = 0; i < 2; ++i) fma_f32x2(acc[l * kLd / 8 + j][h][i], v[l][h][4 * j + 2 * i], v[l][h][4 * j + 2 * i + 1], f2);
             }
-        }
+          }
         if (kq == kScaleBlocks - 1 || kb + 1 == kb1) {
           __syncwarp();
           if (lane == 0) mbar_arrive(sempty(s));
@@ -503,8 +520,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
 }
 
 // ---------------------------------------------------------------------------
-// Many rows per group: 128 token rows x 256 weight rows.  Here the token rows are the M operand (a lane of tensor memory each),
-// so that sa * sb is one number per thread and block.
+// Many rows per group: 128 token rows (a lane of tensor memory each) x 256 weight rows.  Eight epilogue warps: a quadrant of the rows
+// and a half of the columns, which is a row of scale blocks; a warp each for copies, MMAs, and scales and bias.
 // ---------------------------------------------------------------------------
 constexpr int kWideTok = 128, kWideN = 256;
 constexpr int kWideTile = kWideTok * kScaleBlock;                       // bytes of the token rows of a block of k

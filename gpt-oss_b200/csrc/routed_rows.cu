@@ -414,7 +414,8 @@ cudaError_t launch_route_scored(const moe_route_rule &r, const void *logits, siz
 // ranges of pairs and their warps contiguous parts of them, each with a histogram of its own.  Every CTA reads the others'
 // totals from their shared memory; prefixes over experts, CTAs and warps then give every warp its place in every expert's rows,
 // and a second walk over the same pairs hands the places out, so that they ascend with the pair.  Latency is all there is to
-// it: 8192 x 8 pairs 80 us on one CTA, of which 16 walks of a warp over 64 pairs each are left on eight.
+// it: 8192 x 8 pairs of 256 experts 80 us on one CTA, 10.7 on eight (launch and cluster 3, pairs and histograms 2, prefixes and the
+// other CTAs' totals 3, places 2).
 // ---------------------------------------------------------------------------
 constexpr int kGroupThreads = 1024, kGroupWarps = kGroupThreads / 32, kGroupMaxCtas = 8;
 constexpr int kMaxGroupedExperts = 1024;
