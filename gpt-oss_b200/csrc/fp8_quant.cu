@@ -275,9 +275,9 @@ int moe_quantize_fp8(moe_handle c, const void *x_dev, int dtype, long long ld_x,
   if (!x_dev || !codes_dev || !scales_dev) return op_fail(c, MOE_ERR_INVALID, "moe_quantize_fp8: null tensor");
   if (!aligned_to(x_dev, size) || !aligned_to(pair_row_dev, 4) || !aligned_to(n_rows_dev, 4) || !aligned_to(scales_dev, 4))
     return op_fail(c, MOE_ERR_INVALID, "moe_quantize_fp8: a tensor is not aligned to its elements");
-  if (int rc = use_device(c, "moe_quantize_fp8")) return rc;
   const long long units = static_cast<long long>(rows) * n_blocks;
   if (units > 0x3fffffffll) return op_fail(c, MOE_ERR_INVALID, "moe_quantize_fp8: %d rows of %d columns in one call", rows, cols);
+  if (int rc = use_device(c, "moe_quantize_fp8")) return rc;
   // wide accesses: rows of 16-byte pieces (with MOE_ACT_SILU_MUL the second half of a row of x too)
   const int wide_in = aligned_to(x_dev, 16) && ld_x * size % 16 == 0 && (act != MOE_ACT_SILU_MUL || static_cast<long long>(cols) * size % 16 == 0);
   const int wide_out = aligned_to(codes_dev, 16) && ld_codes % 16 == 0;

@@ -270,7 +270,8 @@ int moe_group_pairs(moe_handle h, const int *idx_dev, int rows, int top_k, int n
  * (`cols` counts v; with an activation x has 2 * cols columns).  Row t is written to the fanout rows pair_row_dev[t, 0..fanout)
  * of codes_dev [out_rows, ld_codes] and scales_dev [out_rows, ld_scales >= ceil(cols / 128)]; places outside [0, out_rows) are
  * left out.  Without pair_row_dev row t goes to row t.  n_rows_dev (i32, may be NULL) on the device says how many of the rows
- * exist; rows, and columns behind `cols`, that nothing is written to keep what they hold. */
+ * exist; rows, and columns behind `cols`, that nothing is written to keep what they hold.  rows * ceil(cols / 128) must be below
+ * 2^30 and every stride fit an int.  Rows of 16-byte pieces (x, codes) are read and written in those. */
 int moe_quantize_fp8(moe_handle h, const void *x_dev, int dtype, long long ld_x, int rows, int cols, int act, float limit,
                      float alpha, const int *pair_row_dev, int fanout, int out_rows, const int *n_rows_dev, uint8_t *codes_dev,
                      long long ld_codes, float *scales_dev, long long ld_scales, void *stream);
@@ -285,7 +286,7 @@ int moe_quantize_fp8_blocks(moe_handle h, const void *w_dev, int dtype, long lon
  * b_dev e4m3 [n_groups, n, ld_b], sb_dev [n_groups, ceil(n / 128), ceil(k / 128)], bias_dev bf16 [n_groups, n] or NULL.
  * offsets_dev i32 [n_groups + 1] on the device, ascending: group g (<= 1024) is rows [offsets[g], offsets[g + 1]), output rows
  * in no group keep what they hold; NULL: one group, all rows.  ld_a and ld_b are multiples of 16 and both code tensors 16-byte
- * aligned (MOE_ERR_INVALID otherwise); codes behind column k are not looked at. */
+ * aligned (MOE_ERR_INVALID otherwise); codes behind column k are not looked at.  Output rows of 16-byte pieces are the fastest. */
 int moe_gemm_fp8(moe_handle h, const uint8_t *a_dev, long long ld_a, const float *sa_dev, long long ld_sa, int rows,
                  const uint8_t *b_dev, long long ld_b, const float *sb_dev, int n, int k, int n_groups, const int *offsets_dev,
                  const void *bias_dev, void *out_dev, int out_dtype, long long ld_out, void *stream);

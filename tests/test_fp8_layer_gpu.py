@@ -223,6 +223,32 @@ def test_quantise_rows_bit_for_bit(rows, cols, dtype, pad, shift, pkg, handle):
     assert (far <= v.abs() * (2.0 ** -4 + 2.0 ** -21) + scales.double()[:, torch.arange(cols) // 128] * 2.0 ** -10).all()
 
 
+@pytest.mark.parametrize("act", ["none", "swiglu", "silu"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,cols,fanout", [(1, 128, 1), (3, 300, 2), (70, 1000, 6), (257, 2881, 4)])
+def test_quantise_alignment_does_not_change_results(rows, cols, fanout, dtype, act, pkg, handle):
+    """Rows of x at any element, codes in 16-byte rows or not: the same codes and scales, bit for bit."""
+    wide = cols if act == "none" else 2 * cols
+    g = gen(rows + cols)
+    aligned = torch.zeros(rows, ref.pad16(wide), device="cuda", dtype=TYPES[dtype])
+    aligned[:, :wide] = 4 * randn(g, rows, wide)
+    odd = torch.zeros(rows * (wide + 3) + 1, device="cuda", dtype=TYPES[dtype])[1:].view(rows, wide + 3)
+    odd[:, :wide] = aligned[:, :wide]
+    place = torch.randperm(rows * fanout, generator=g, device="cuda").int().view(rows, fanout).contiguous()
+    results = []
+    for x in (aligned, odd):
+        for ld, shift in ((ref.pad16(cols), 0), (ref.pad16(cols) + 3, 1)):
+            codes, scales = run_quantise(pkg, handle, x, cols, act=act, dtype=dtype, pair_row=place, out_rows=rows * fanout, ld_codes=ld, shift=shift)
+            assert (codes[:, cols:] == 0x55).all()
+            results.append((codes[:, :cols], scales))
+    for codes, scales in results[1:]:
+        assert torch.equal(codes, results[0][0]) and torch.equal(scales, results[0][1])
+    if act == "none":
+        want, want_s = ref.quantise_rows(aligned[:, :cols])
+        assert torch.equal(results[0][0][place.long().flatten()], want.view(torch.uint8).repeat_interleave(fanout, 0))
+        assert torch.equal(results[0][1][place.long().flatten()], want_s.repeat_interleave(fanout, 0))
+
+
 def test_quantise_extreme_values(pkg, handle):
     x = randn(gen(1), 8, 256)
     x[0] = 0
@@ -372,7 +398,7 @@ def test_product_output_types_and_strides(rows, out, pad, pkg, handle):
 
 GROUPED = [([1], 96, 200), ([0, 0, 5, 0], 300, 256), ([8] * 8, 384, 512), ([3, 0, 17, 1, 0, 64, 2, 9], 260, 1040), ([130, 1, 0, 127, 128, 129], 520, 384),
            ([700, 5, 0, 300, 33], 256, 640), ([0, 0, 0], 128, 128), ([1] * 40, 144, 2880), ([257, 255, 256, 0, 31, 32, 33], 1152, 128),
-           ([16] * 200, 64, 64)]
+           ([16] * 200, 64, 64), ([1700, 5, 0, 2300, 33], 520, 384), ([1] * 1024, 130, 144)]
 
 
 @pytest.mark.parametrize("counts,n,k", GROUPED)
@@ -384,6 +410,18 @@ def test_grouped_product(counts, n, k, out, extra, pkg, handle):
         p["rows"] = 4
         p = {**p, "a": codes_of(gen(1), 1.0, 4, k), "sa": torch.ones(4, ref.blocks(k), device="cuda")}
     check_product(p, run_product(pkg, handle, p, out), out)
+
+
+@pytest.mark.parametrize("rows,first", [(60, 7), (700, 130)])
+def test_rows_before_the_first_group_stay(rows, first, pkg, handle):
+    p = make_product(3, rows, 200, 260, groups=2, counts=[rows // 2 - first, rows // 2])
+    p["offsets"] = p["offsets"] + first
+    buf = run_product(pkg, handle, p, "f32")
+    want, mag = ref.gemm(p["a"][:, :260].contiguous().view(torch.float8_e4m3fn), p["sa"], p["b"][:, :, :260].contiguous().view(torch.float8_e4m3fn), p["sb"],
+                         p["offsets"])
+    last = int(p["offsets"][-1])
+    assert ((buf.double() - want).abs() <= half_step(want, "f32") + mag * 131 * 2.0 ** -23)[first:last].all()
+    assert (buf[:first] == 77).all() and (buf[last:] == 77).all()
 
 
 @pytest.mark.parametrize("rows,counts", [(20, None), (400, None), (200, [120, 0, 80])])
@@ -588,3 +626,36 @@ def test_layer_in_a_graph_beside_a_layer_on_another_stream(pkg, handle):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, o) and torch.equal(ob, want_b)
+
+
+def test_first_calls_of_a_handle_are_captured_across_streams(pkg):
+    """A handle whose first calls are made under capture, on two streams that fork and join."""
+    h = pkg.MoeBlock(64, 64, 8, max_rows=8)
+    try:
+        small, large = make_product(1, 12, 260, 1024, bias=True), make_product(2, 300, 260, 1024, bias=True)
+        idx = torch.randint(0, 40, (500, 4), generator=gen(5), device="cuda", dtype=torch.int32)
+        offsets, pair_row, row_pair = torch.zeros(41, dtype=torch.int32, device="cuda"), torch.zeros_like(idx), torch.zeros(2000, dtype=torch.int32, device="cuda")
+        outs = [torch.zeros(p["rows"], 260, device="cuda") for p in (small, large)]
+        side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+
+        def product(p, buf):
+            h.gemm_fp8(p["a"].data_ptr(), p["a"].shape[1], p["sa"].data_ptr(), p["sa"].shape[1], p["rows"], p["b"].data_ptr(), p["b"].shape[2],
+                       p["sb"].data_ptr(), p["n"], p["k"], buf.data_ptr(), pkg.F32, 260, bias_ptr=p["bias"].data_ptr(), stream=stream())
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            h.group_pairs(idx.data_ptr(), 500, 4, 40, offsets.data_ptr(), pair_row.data_ptr(), row_pair.data_ptr(), stream())
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                product(small, outs[0])
+            product(large, outs[1])
+            torch.cuda.current_stream().wait_stream(side)
+            h.group_pairs(idx.data_ptr(), 500, 4, 40, offsets.data_ptr(), pair_row.data_ptr(), 0, stream())
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, want in zip((offsets, pair_row, row_pair), ref.group(idx, 40)):
+            assert torch.equal(got.cpu(), want)
+        for p, buf in zip((small, large), outs):
+            check_product(p, buf, "f32")
+        h.synchronize()
+    finally:
+        h.close()

@@ -69,7 +69,8 @@ QUANT = dict(x=P, dtype=1, ld_x=256, rows=4, cols=256, act=0, limit=7.0, alpha=1
     dict(x=0), dict(codes=0), dict(scales=0), dict(dtype=3), dict(ld_x=255), dict(rows=-1), dict(cols=0), dict(ld_codes=255), dict(ld_scales=1),
     dict(act=3), dict(act=1), dict(act=1, ld_x=512, limit=-1.0), dict(act=1, ld_x=512, limit=float("nan")), dict(act=1, ld_x=512, alpha=float("inf")),
     dict(fanout=0), dict(fanout=2), dict(out_rows=3), dict(out_rows=-1, pair_row=P), dict(pair_row=P, fanout=1 << 30), dict(x=P + 1), dict(scales=P + 2),
-    dict(pair_row=P + 2, fanout=2), dict(n_rows=P + 3)])
+    dict(pair_row=P + 2, fanout=2), dict(n_rows=P + 3), dict(ld_x=1 << 31), dict(ld_codes=1 << 31), dict(ld_scales=1 << 31),
+    dict(rows=1 << 30, out_rows=1 << 30)])
 def test_quantise(change, pkg, handle):
     refused(pkg, handle, pkg.lib().moe_quantize_fp8(handle, *{**QUANT, **change}.values(), None), "moe_quantize_fp8")
 
