@@ -18,8 +18,10 @@ namespace moe {
 // is off by less than 2^-21 (s (1 - s) times the exponential's (2 + 1.2 |x|) 2^-23, and the roundings of sum and quotient), a
 // softmax by less than 2^-18 of the row's largest (exponentials, a sum of up to 512, a quotient); so an order is certain where two
 // values differ by 2^-20, or 2^-17 of that largest, and 2^-22 of their own magnitudes (twice that for sums of two), or where
-// both logits and both biases are equal: then the index decides.  A row with a closer call is done again in 64 bits, in
-// code that is cold: 3 us more for a call of 8192 rows, however few they are.
+// both logits and both biases are equal: then the index decides.  A row with a closer call is done again in 64 bits.  Of 8192 rows
+// of 256 experts some 18 are: 10.4 us without them, 15.2 with them, which is the time of one such row at the end (code that is not
+// in the instruction cache, eight rounds on 64-bit keys 1.6 us, the exponentials 0.3).  Settling only the calls in doubt, with one
+// exponential a lane, took the same 15.2, and 0.6 us more on a single row.
 //
 // A warp per row; lane l owns the per_lane consecutive experts from l * per_lane, so that a lower lane is a lower index.
 // ---------------------------------------------------------------------------
@@ -59,15 +61,9 @@ __device__ __forceinline__ R warp_sum(R v) {
   return v;
 }
 
-// The two largest keys of every group, in all of its lanes: a group is `lanes` whole lanes, a power of two.
-template <class Key, int kPer>
-__device__ __forceinline__ void two_best(const Key (&key)[kPer], int lanes, Key &k1, Key &k2) {
-  k1 = k2 = 0;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    k2 = max(k2, min(k1, key[i]));
-    k1 = max(k1, key[i]);
-  }
+// The two largest keys of a lane -> those of its group, in all of the group's lanes: `lanes` whole ones, a power of two.
+template <class Key>
+__device__ __forceinline__ void two_best(int lanes, Key &k1, Key &k2) {
   for (int off = 1; off < lanes; off <<= 1) {
     const Key o1 = __shfl_xor_sync(0xffffffffu, k1, off), o2 = __shfl_xor_sync(0xffffffffu, k2, off);
     k2 = max(max(k2, o2), min(k1, o1));
@@ -112,13 +108,35 @@ __device__ __forceinline__ Key take_best(Key (&key)[kPer], Key &best, int lane, 
   return top;
 }
 
+// Largest first, by a network of fixed comparisons (odd-even merges).
+template <int kPer>
+__device__ __forceinline__ void sort_keys(unsigned (&key)[kPer]) {
+#pragma unroll
+  for (int p = 1; p < kPer; p *= 2)
+#pragma unroll
+    for (int d = p; d >= 1; d /= 2)
+#pragma unroll
+      for (int a = 0; a + d < kPer; ++a)
+        if (a >= d % p && (a - d % p) % (2 * d) < d && a / (2 * p) == (a + d) / (2 * p)) {
+          const unsigned low = min(key[a], key[a + d]);
+          key[a] = max(key[a], key[a + d]);
+          key[a + d] = low;
+        }
+}
+
 // One row in 32 bits.  x[i]: the lane's logits, -inf where there is none; b[i]: its biases, -inf where there is no expert.  Lane
 // k < top_k receives the k-th selected expert (or -1) in `sel`.  `top` and `sum`: of the softmax.  Returns false where 32 bits do
 // not settle a comparison.  Groups are `group_lanes` whole lanes.
+//
+// The low bits of a key give way to the place in the lane (a lower place is a higher key), and a lane sorts its keys once: a round
+// of the selection is then a maximum over the lanes' first keys and a shift in the lane that has it.  With unsorted keys, of
+// which a round looked for its winner again, 8192 rows of 256 experts took 17.5 us instead of 15.2.
 template <class T, int kPer>
 __device__ __forceinline__ bool select_fast(const T *src, const float (&x)[kPer], const float *bias, const float (&b)[kPer], const moe_route_rule &rule,
                                             int per_lane, int group_lanes, int lane, float top, float &sum, int &sel) {
   const float inf = __int_as_float(0x7f800000);
+  constexpr unsigned kPlace = kPer - 1;       // bits of a place
+  constexpr bool kExact = sizeof(T) == 2;     // logits whose keys lose nothing to the place
   const bool softmax = rule.score == MOE_SCORE_SOFTMAX;
   auto score = [&](float v) { return softmax ? __expf(v - top) : __fdividef(1.f, 1.f + __expf(-v)); };
   float over = 1.f;   // a softmax is score * over
@@ -145,40 +163,51 @@ __device__ __forceinline__ bool select_fast(const T *src, const float (&x)[kPer]
     for (int i = 0; i < kPer; ++i) key[i] = ordered_key(x[i]);
   }
 #pragma unroll
-  for (int i = 0; i < kPer; ++i)
-    if (!(x[i] > -inf) || !(b[i] > -inf)) key[i] = 0;
-  const float close = softmax ? over * 7.62939453125e-06f : 9.5367431640625e-07f, rel = 2.384185791015625e-07f;   // 2^-17, 2^-20, 2^-22
+  for (int i = 0; i < kPer; ++i) key[i] = x[i] > -inf && b[i] > -inf ? (key[i] & ~kPlace) | (kPlace - i) : 0;   // (a finite value's key is above 2^22)
+  sort_keys(key);
+  // what a key stands for, off by less than `lost` of its magnitude (towards zero)
+  auto value = [&](unsigned k) { return __uint_as_float(((k >> 31) ? k & 0x7fffffffu : ~k) & ~kPlace); };
+  constexpr float lost = kPlace * 1.1920928955078125e-07f;                        // 2^-23 a place
+  constexpr float rel = lost + 2.384185791015625e-07f;                            // and 2^-22
+  const float close = softmax ? over * 7.62939453125e-06f : 9.5367431640625e-07f;   // 2^-17, 2^-20
   auto far_apart = [&](float a, float c, float twice) { return a - c > twice * (close + rel * (fabsf(a) + fabsf(c))); };
   // the order of two keys (the first is not the smaller) is that of 64 bits
   auto certain = [&](unsigned ka, unsigned kc) {
-    const float a = key_value(ka), c = key_value(kc);
+    const float a = value(ka), c = value(kc);
     if (bias != nullptr) return far_apart(a, c, 1.f);
-    const bool resolved = softmax ? c > top - 600.f : a < 16.f && c > -600.f;
-    return resolved && (ka == kc || a - c > 1e-9f);
+    return (softmax ? a > top - 600.f : c < 16.f && a > -600.f) && a - c > 1e-9f + (kExact ? 0.f : lost * (fabsf(a) + fabsf(c)));
   };
   bool settled = true;
   if (rule.n_groups > 1) {
-    unsigned k1, k2;
-    two_best(key, group_lanes, k1, k2);
-    k1 = __shfl_sync(0xffffffffu, k1, lane * group_lanes & 31);   // lane g: those of group g
-    k2 = __shfl_sync(0xffffffffu, k2, lane * group_lanes & 31);
+    unsigned k1 = key[0], k2 = kPer > 1 ? key[kPer > 1 ? 1 : 0] : 0;
+    two_best(group_lanes, k1, k2);
+    k1 = __shfl_sync(0xffffffffu, k1, lane * group_lanes & 31) & ~kPlace;   // lane g: those of group g
+    k2 = __shfl_sync(0xffffffffu, k2, lane * group_lanes & 31) & ~kPlace;
     if (lane >= rule.n_groups) k1 = k2 = 0;
     unsigned worth = k1;
+    float off = 0.f;   // how far a sum may be off for what its logits lost
     const bool sums = rule.group_top == 2;
     if (sums && k1 != 0) {
-      auto value = [&](unsigned k) { return k == 0 ? 0.f : bias != nullptr ? key_value(k) : score(key_value(k)) * over; };
-      worth = ordered_key(value(k1) + value(k2));
+      auto part = [&](unsigned k) {
+        if (k == 0) return 0.f;
+        const float v = value(k);
+        if (bias != nullptr) return v;
+        const float s = score(v) * over, d = lost * fabsf(v);
+        if (!kExact) off += d < 0.1f ? 1.1f * d * s : inf;
+        return s;
+      };
+      worth = ordered_key(part(k1) + part(k2));
     }
     const int rank = group_rank(worth, rule.n_groups, lane);
     const unsigned stays = __ballot_sync(0xffffffffu, rank < rule.top_groups);
-    if (rule.top_groups < rule.n_groups) {   // the last group that stays against the first that does not
-      const int in = __ffs(__ballot_sync(0xffffffffu, rank == rule.top_groups - 1)) - 1, out = __ffs(__ballot_sync(0xffffffffu, rank == rule.top_groups)) - 1;
+    if (rule.top_groups < rule.n_groups) {   // every group against the last that stays: above it, below it, or made of the same
+      const int in = __ffs(__ballot_sync(0xffffffffu, rank == rule.top_groups - 1)) - 1;
       const unsigned a1 = __shfl_sync(0xffffffffu, k1, in), a2 = __shfl_sync(0xffffffffu, k2, in), wa = __shfl_sync(0xffffffffu, worth, in);
-      const unsigned c1 = __shfl_sync(0xffffffffu, k1, out), c2 = __shfl_sync(0xffffffffu, k2, out), wc = __shfl_sync(0xffffffffu, worth, out);
-      if (wc != 0) {
-        if (!sums) settled = certain(a1, c1);
-        else if (bias == nullptr && a1 == c1 && a2 == c2) settled = true;
-        else settled = far_apart(key_value(wa), key_value(wc), 2.f);
+      const float off_in = __shfl_sync(0xffffffffu, off, in);
+      if (worth != 0 && wa != 0) {
+        const unsigned hi = max(worth, wa), lo = min(worth, wa);
+        const bool same = lane == in || (kExact && bias == nullptr && k1 == a1 && (!sums || k2 == a2));
+        settled = same || (sums ? far_apart(key_value(hi) - off - off_in, key_value(lo), 2.f) : certain(hi, lo));
       }
     }
     if (!(stays >> (lane / group_lanes) & 1u)) {
@@ -186,29 +215,32 @@ __device__ __forceinline__ bool select_fast(const T *src, const float (&x)[kPer]
       for (int i = 0; i < kPer; ++i) key[i] = 0;
     }
   }
-  // one round more than experts, for the first that is not selected: lane k keeps the k-th, and neighbours are compared at the end
-  sel = -1;
-  unsigned best = key[0], kept = 0, beyond = 0;
+  // lane k keeps the k-th; the lowest lane wins among equal ones
+  unsigned kept = 0;
+  int from = 0;
+  for (int k = 0; k < rule.top_k; ++k) {
+    const unsigned best = __reduce_max_sync(0xffffffffu, key[0]);
+    if (best == 0) break;
+    const int owner = __ffs(__ballot_sync(0xffffffffu, (key[0] ^ best) <= kPlace)) - 1;
+    const unsigned won = __shfl_sync(0xffffffffu, key[0], owner);
+    if (lane == k) { kept = won; from = owner; }
+    if (lane == owner) {
 #pragma unroll
-  for (int i = 1; i < kPer; ++i) best = max(best, key[i]);
-  int next_sel = -1;   // of lane 31: the expert of round 32
-  for (int k = 0; k <= rule.top_k; ++k) {
-    int at, owner;
-    const unsigned top_key = take_best(key, best, lane, at, owner);
-    if (top_key == 0) break;
-    const int e = owner * per_lane + at;
-    if (lane == k) { kept = top_key; sel = e; }
-    if (k == 32) { beyond = top_key; next_sel = e; }
+      for (int i = 0; i + 1 < kPer; ++i) key[i] = key[i + 1];
+      key[kPer - 1] = 0;
+    }
   }
-  unsigned after = __shfl_down_sync(0xffffffffu, kept, 1);
-  int after_sel = __shfl_down_sync(0xffffffffu, sel, 1);
-  if (lane == 31) { after = beyond; after_sel = next_sel; }
-  if (lane < rule.top_k && kept != 0 && after != 0 && !certain(kept, after)) {
-    // equal logits under equal biases: the index has decided
-    const bool same = bias != nullptr && to_f32(src[sel]) == to_f32(src[after_sel]) && bias[sel] == bias[after_sel];
-    if (!same) settled = false;
+  sel = kept != 0 ? from * per_lane + static_cast<int>(kPlace - (kept & kPlace)) : -1;
+  // neighbours among the selected, and the last of them against all that is left.  Equal logits under equal biases: the index decided
+  auto same = [&](int e, int f) { return to_f32(src[e]) == to_f32(src[f]) && (bias == nullptr || bias[e] == bias[f]); };
+  const unsigned after = __shfl_down_sync(0xffffffffu, kept, 1), last = __shfl_sync(0xffffffffu, kept, rule.top_k - 1);
+  const int after_sel = __shfl_down_sync(0xffffffffu, sel, 1), last_sel = __shfl_sync(0xffffffffu, sel, rule.top_k - 1);
+  if (lane + 1 < rule.top_k && after != 0 && !certain(kept, after) && !same(sel, after_sel)) settled = false;
+  if (key[0] != 0 && !certain(last, key[0])) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (key[i] != 0 && !certain(last, key[i]) && !same(last_sel, lane * per_lane + static_cast<int>(kPlace - (key[i] & kPlace)))) settled = false;
   }
-  if (lane >= rule.top_k) sel = -1;
   return __all_sync(0xffffffffu, settled);
 }
 
@@ -245,7 +277,12 @@ __device__ __forceinline__ void select_exact(const float (&x)[kPer], const float
     const int size = rule.n_experts / rule.n_groups;
     Key k1 = 0, k2 = 0;
     if (group_lanes > 0) {
-      two_best(key, group_lanes, k1, k2);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        k2 = max(k2, min(k1, key[i]));
+        k1 = max(k1, key[i]);
+      }
+      two_best(group_lanes, k1, k2);
     } else {
 #pragma unroll
       for (int i = 0; i < kPer; ++i)

@@ -129,6 +129,24 @@ def test_route_next_to_a_tie_is_decided_in_64_bits(pkg, handle):
 
 
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts,groups,group_top,top_k", [(256, 1, 1, 8), (256, 8, 2, 8), (64, 8, 1, 6), (512, 4, 2, 32), (30, 1, 1, 4)])
+@pytest.mark.parametrize("bias", ["none", "zero", "steps"])
+def test_route_values_a_few_steps_apart(score, experts, groups, group_top, top_k, bias, pkg, handle):
+    """Rows of few levels, every value of a level some last places off, with exact ties among them.  Sums of two differ by the
+    second order of a step, 4e-15 at the upper levels, ten last places of 64 bits; under a bias that few values share, sums of
+    the same parts in another pairing would not, so every expert has its own there."""
+    g = gen(experts + groups)
+    levels = torch.tensor([-3.0, -0.5, 0.25, 1.0, 1.5, 2.0, 2.5], device="cuda")
+    level = levels[torch.randint(0, 7, (400, experts), generator=g, device="cuda")]
+    x = level * (1 + torch.randint(0, 40, (400, experts), generator=g, device="cuda") * 2.0 ** -23)
+    b = {"none": None, "zero": torch.zeros(experts, device="cuda"),
+         "steps": 0.125 + 2.0 ** -20 * (randn(g, experts) if group_top == 2 else torch.randint(0, 3, (experts,), generator=g, device="cuda"))}[bias]
+    top_groups = max(1, groups // 2)
+    got = run_route(pkg, handle, x, b, top_k, score, groups, top_groups, group_top)
+    check_route(got, ref.route(x, b, top_k, score, groups, top_groups, group_top))
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("groups,group_top", [(1, 1), (8, 1), (8, 2)])
 @pytest.mark.parametrize("bias", ["none", "zero", "steps"])
 def test_route_many_equal_scores(score, groups, group_top, bias, pkg, handle):
