@@ -72,9 +72,9 @@ __device__ __forceinline__ float gated(float gate, float up, float limit, float 
 template <class T>
 struct Raw16 {
   uint4 v[sizeof(T)];
-  __device__ __forceinline__ void load(const T *p) {
+  __device__ __forceinline__ void load(const T *p, bool there) {
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T)); ++i) v[i] = reinterpret_cast<const uint4 *>(p)[i];
+    for (int i = 0; i < static_cast<int>(sizeof(T)); ++i) v[i] = there ? reinterpret_cast<const uint4 *>(p)[i] : make_uint4(0, 0, 0, 0);
   }
   __device__ __forceinline__ void load_spread(const T *p, int n, int step) {
     T *e = reinterpret_cast<T *>(v);
@@ -120,12 +120,12 @@ __device__ __forceinline__ float finite_max(const float (&v)[16], float m) {
 
 // Eight lanes per block of 128 columns, sixteen columns each; the (row, block) pairs of a call are dealt to the groups of lanes.
 // Bound by instructions (addresses, places, the two quotients of a block cost the same whatever a lane converts): with eight
-// columns a lane 6144 x 2880 values through SwiGLU took 24 us, 1856 rows to four places each 8.5 us.  More pairs of a thread
-// under way together cost registers and time.
+// columns a lane 6144 x 2880 values through SwiGLU took 24 us, 1856 rows to four places each 8.5 us; they take 20.0 and 6.7.  More
+// pairs of a thread under way together cost registers and time; four CTAs to an SM in place of five 21.5 us.
 constexpr int kQuantThreads = 256, kQuantGroups = kQuantThreads / kQuantLanes, kPlaces = 4;
 
 template <class T, int kAct, bool kWideIn>
-__global__ void __launch_bounds__(kQuantThreads)
+__global__ void __launch_bounds__(kQuantThreads, 5)
 quantize_fp8_kernel(const T *x, unsigned ld_x, int rows, int cols, unsigned n_blocks, float limit, float rate, const int *pair_row, unsigned fanout,
                     int out_rows, const int *n_rows, uint8_t *codes, unsigned ld_codes, float *scales, unsigned ld_scales, int wide_out) {
   grid_dep_sync();
@@ -138,10 +138,10 @@ quantize_fp8_kernel(const T *x, unsigned ld_x, int rows, int cols, unsigned n_bl
   for (unsigned unit = blockIdx.x * kQuantGroups + threadIdx.x / kQuantLanes; __any_sync(0xffffffffu, unit < units); unit += stride) {
     const bool on = unit < units;
     const unsigned row = on ? unit / n_blocks : 0, kb = on ? unit - row * n_blocks : n_blocks;   // no column of block n_blocks exists
-    // a lane's columns: sixteen neighbours, or, where rows of x are not 16-byte aligned and in a row's last part of a block, every
-    // eighth
+    // a lane's columns: sixteen neighbours, or, where rows of x are not 16-byte aligned and in a last part of a block that is not made
+    // of sixteens, every eighth
     const int left = cols - static_cast<int>(kb * kScaleBlock);
-    const bool whole = kWideIn && wide_out && left >= kScaleBlock;
+    const bool packed_out = wide_out && (left >= kScaleBlock || cols % kQuantCols == 0), whole = kWideIn && packed_out;
     const int c0 = static_cast<int>(kb * kScaleBlock + lane * (whole ? kQuantCols : 1)), n = cols - c0;
     const T *src = x + static_cast<size_t>(row) * ld_x;
     float v[16];
@@ -153,7 +153,7 @@ quantize_fp8_kernel(const T *x, unsigned ld_x, int rows, int cols, unsigned n_bl
     }
     if (kAct == MOE_ACT_NONE) {
       Raw16<T> a;
-      if (whole) a.load(src + c0);
+      if (whole) a.load(src + c0, n > 0);
       else a.load_spread(src + c0, n, kQuantLanes);
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] = a[i];
@@ -164,11 +164,11 @@ quantize_fp8_kernel(const T *x, unsigned ld_x, int rows, int cols, unsigned n_bl
         a.load_spread(src + at, n, step);
         b.load_spread(src + at + (kAct == MOE_ACT_SWIGLU ? 1 : cols), n, step);
       } else if (kAct == MOE_ACT_SWIGLU) {
-        a.load(src + 2 * c0);
-        b.load(src + 2 * c0 + 16);
+        a.load(src + 2 * c0, n > 0);
+        b.load(src + 2 * c0 + 16, n > 0);
       } else {
-        a.load(src + c0);
-        b.load(src + cols + c0);
+        a.load(src + c0, n > 0);
+        b.load(src + cols + c0, n > 0);
       }
       if (kAct == MOE_ACT_SWIGLU && whole) {
 #pragma unroll
@@ -183,17 +183,16 @@ quantize_fp8_kernel(const T *x, unsigned ld_x, int rows, int cols, unsigned n_bl
     }
     const float m = block_max(finite_max(v, kAmaxFloor));
     uint4 q = encode16(v, __fdiv_rn(kFp8Max, m));
-    if (!kWideIn && wide_out) {   // (all lanes: a full block among the warp's is reason enough)
+    if (!kWideIn && wide_out) {   // (all lanes: one block of the warp's is reason enough)
       const uint4 packed = gather_codes(q);
-      if (left >= kScaleBlock) q = packed;
+      if (packed_out) q = packed;
     }
-    const bool packed_out = wide_out && left >= kScaleBlock;
     const float scale = __fdiv_rn(m, kFp8Max);
     auto put = [&](int r) {
       if (static_cast<unsigned>(r) >= static_cast<unsigned>(out_rows)) return;
       uint8_t *dst = codes + static_cast<size_t>(static_cast<unsigned>(r)) * ld_codes;
-      if (packed_out) *reinterpret_cast<uint4 *>(dst + kb * kScaleBlock + lane * kQuantCols) = q;
-      else write_spread(dst + c0, n, q);
+      if (!packed_out) write_spread(dst + c0, n, q);
+      else if (static_cast<int>(lane * kQuantCols) < left) *reinterpret_cast<uint4 *>(dst + kb * kScaleBlock + lane * kQuantCols) = q;
       if (lane == 0) scales[static_cast<size_t>(static_cast<unsigned>(r)) * ld_scales + kb] = scale;
     };
 #pragma unroll
@@ -212,7 +211,7 @@ quantize_fp8_blocks_kernel(const T *w, size_t ld_w, int rows, int cols, uint8_t 
   constexpr int kRows = kScaleBlock / kQuantGroups;   // of a thread
   const int lane = threadIdx.x % kQuantLanes, group = threadIdx.x / kQuantLanes;
   const int r0 = blockIdx.y * kScaleBlock;
-  const bool whole = wide && cols - static_cast<int>(blockIdx.x * kScaleBlock) >= kScaleBlock;   // (quantize_fp8_kernel)
+  const bool whole = wide && (cols - static_cast<int>(blockIdx.x * kScaleBlock) >= kScaleBlock || cols % kQuantCols == 0);   // (quantize_fp8_kernel)
   const int c0 = blockIdx.x * kScaleBlock + lane * (whole ? kQuantCols : 1), n = cols - c0;
   const size_t mat = blockIdx.z;
   const T *src = w + mat * rows * ld_w;
@@ -222,7 +221,7 @@ quantize_fp8_blocks_kernel(const T *w, size_t ld_w, int rows, int cols, uint8_t 
   for (int j = 0; j < kRows; ++j) {
     const int r = r0 + group + kQuantGroups * j;
     const T *from = src + static_cast<size_t>(min(r, rows - 1)) * ld_w + c0;   // (a row again, where there is none: no other maximum)
-    if (whole) raw[j].load(from);
+    if (whole) raw[j].load(from, n > 0);
     else raw[j].load_spread(from, n, kQuantLanes);
   }
   float v[16];
@@ -246,8 +245,8 @@ quantize_fp8_blocks_kernel(const T *w, size_t ld_w, int rows, int cols, uint8_t 
     for (int i = 0; i < 16; ++i) v[i] = raw[j][i];
     if (r >= rows) continue;
     uint8_t *dst = codes + (mat * rows + r) * ld_codes + c0;
-    if (whole) *reinterpret_cast<uint4 *>(dst) = encode16(v, inv);
-    else write_spread(dst, n, encode16(v, inv));
+    if (!whole) write_spread(dst, n, encode16(v, inv));
+    else if (n > 0) *reinterpret_cast<uint4 *>(dst) = encode16(v, inv);
   }
   if (threadIdx.x == 0) scales[(mat * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x] = __fdiv_rn(m, kFp8Max);
 }
