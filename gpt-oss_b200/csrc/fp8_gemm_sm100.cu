@@ -17,7 +17,7 @@
 // scales then serves four packed multiply-adds.  With a row per thread every scale of the tile is loaded in every thread, and a
 // block of 128 x 128 took 700 cycles for its multiply-adds instead of 120, although the tensor-memory loads of fragments are
 // slower (128 cycles of a quadrant for 64 columns, 35 for rows).  Bound by HBM: 256 rows over 32 experts of 5760 x 2880 85 us =
-// 6.3 TB/s.  One decode step (16 x 4096 x 7168) 8.7 us for the 4.5 that its weights take: launch, 14 blocks of k, and the sum
+// 6.3 TB/s.  One decode step (16 x 4096 x 7168) 8.6 us for the 4.5 that its weights take: launch, 14 blocks of k, and the sum
 // of four CTAs' parts.
 //
 // Many rows per group (fp8_gemm_wide_kernel).  128 token rows x 256 weight rows; the token rows are the M operand, so that sa * sb
@@ -123,11 +123,12 @@ struct GemmTile {
   int g, nb, row0, ntok;
 };
 
-// A CTA's share of a split tile, kWidth output columns from n0: rows split, split + splits, ..., `mine` of them.  Four places of a
-// thread are under way together: a load from another CTA's shared memory takes about a microsecond.
-template <int kWidth, int kThreads>
+// A CTA's share of a split tile, kWidth output columns from n0: rows split, split + splits, ..., `mine` of them.  kAhead places of a
+// thread are under way together: a load from another CTA's shared memory takes about a microsecond.  The few rows of the narrow
+// kernel want less code instead: 128 x 4096 x 7168 13.6 us with one place, 14.2 with four.
+template <int kWidth, int kThreads, int kAhead>
 __device__ __forceinline__ void add_up_splits(const Fp8GemmArgs &p, const GemmTile &t, uint32_t part, int pitch, int mine, int split, int n0, int out_bytes) {
-  constexpr int kQuads = kWidth / 4, kAhead = 4;
+  constexpr int kQuads = kWidth / 4;
   for (int e0 = threadIdx.x; e0 < mine * kQuads; e0 += kAhead * kThreads) {
     float4 v[kAhead][kMaxSplits];
 #pragma unroll
@@ -153,14 +154,15 @@ __device__ __forceinline__ void add_up_splits(const Fp8GemmArgs &p, const GemmTi
         for (int j = 0; j < 4; ++j) o[j] += n + j < p.n ? __bfloat162float(bias[j]) : 0.f;
       }
       const size_t at = static_cast<size_t>(t.row0 + row) * p.ld_out + n;
-      if (out_bytes == 16 && n + 4 <= p.n) {
-        if (p.out_dtype == MOE_F32) *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at) = make_float4(o[0], o[1], o[2], o[3]);
-        else if (p.out_dtype == MOE_BF16) *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + at) = make_uint2(pack2<__nv_bfloat16>(o[0], o[1]), pack2<__nv_bfloat16>(o[2], o[3]));
-        else *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + at) = make_uint2(pack2<__half>(o[0], o[1]), pack2<__half>(o[2], o[3]));
-      } else {
+      if (p.out_dtype == MOE_F32) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (n + j < p.n) store_out(p, at + j, o[j]);
+          if (n + j < p.n) static_cast<float *>(p.out)[at + j] = o[j];
+      } else {
+        uint16_t *dst = static_cast<uint16_t *>(p.out) + at;
+#pragma unroll
+        for (int j = 0; j < 4; j += 2)
+          store_word16(dst + j, p.out_dtype == MOE_BF16 ? pack2<__nv_bfloat16>(o[j], o[j + 1]) : pack2<__half>(o[j], o[j + 1]), p.n - n - j, out_bytes);
       }
     }
   }
@@ -202,6 +204,8 @@ __device__ __forceinline__ void count_tiles(const Fp8GemmArgs &p, int *s_tiles) 
 // 16 rows; none is empty.
 constexpr int kRunTiles = 12;
 __device__ __forceinline__ GemmTile tile_at(const Fp8GemmArgs &p, const int *s_tiles, int item, int n_nb) {
+  // (every role finds its first tile before anything else can happen: the divisions below are half a microsecond of a decode step)
+  if (p.n_groups == 1 && s_tiles[1] == 1) return GemmTile{0, item, group_begin(p, 0), group_end(p, 0) - group_begin(p, 0)};
   const int q = item / n_nb;
   int lo = 0, hi = p.n_groups;   // s_tiles[lo] <= q < s_tiles[hi]
   while (hi - lo > 1) {
@@ -212,9 +216,13 @@ __device__ __forceinline__ GemmTile tile_at(const Fp8GemmArgs &p, const int *s_t
   const int local = item - s_tiles[lo] * n_nb;
   const int begin = group_begin(p, lo), cnt = group_end(p, lo) - begin;
   const int per = ((cnt + tiles - 1) / tiles + 15) / 16 * 16;
+  if (tiles <= kRunTiles) {
+    const int nb = local / tiles, row = (local - nb * tiles) * per;
+    return GemmTile{lo, nb, begin + row, min(per, cnt - row)};
+  }
   const int run = local / (kRunTiles * n_nb), in_run = local - run * kRunTiles * n_nb, width = min(kRunTiles, tiles - run * kRunTiles);
-  const int row = (run * kRunTiles + in_run % width) * per;
-  return GemmTile{lo, in_run / width, begin + row, min(per, cnt - row)};
+  const int nb = in_run / width, row = (run * kRunTiles + in_run - nb * width) * per;
+  return GemmTile{lo, nb, begin + row, min(per, cnt - row)};
 }
 
 template <int kTok>
@@ -436,8 +444,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
       if (lane == 0) mbar_arrive(pempty(plan));
       if (plan ^= 1u; plan == 0) ppar ^= 1u;
       if (p.out_dtype != MOE_F32) {
-        // 16-bit outputs: blocks of 8 tokens x 32 weight rows are transposed in shared memory and leave as 16 bytes a lane (out_bytes),
-        // or as the 4 or 2 that the output's rows are aligned to
+        // 16-bit outputs: blocks of 8 tokens x 32 weight rows are transposed in shared memory and leave as 16 bytes a lane, or as 4 (2
+        // where the output's rows are not aligned to that)
         const uint32_t stage = ring + S::kOutOff + warp * S::kOutWarp;
         const uint32_t st_at = stage + (lane & 7) * S::kOutPitch + (lane >> 3) * 16;
         const int ntok = t.ntok - col0;
@@ -457,29 +465,33 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
             stmatrix_trans_x4(st_at + j * 8 * S::kOutPitch, w[0], w[1], w[2], w[3]);
           }
           __syncwarp();
-          uint16_t *out = static_cast<uint16_t *>(p.out) + static_cast<size_t>(t.row0 + col0 + 8 * j0) * p.ld_out + n_w;
-          const int here = min(ntok - 8 * j0, S::kOutCols);
-          if (out_bytes == 16) {
-            const int n = (lane & 3) * 8;
-            for (int tok = lane >> 2; tok < here; tok += 8) {
+          // (32 experts of 1440 x 2880: 48 rows each 33.4 us with 16 bytes, 35.4 with 4; but 32 rows each, in the smaller form, 34.1 and
+          // 32.8, and 64 x 4096 x 7168 11.3 and 10.7: there the code's size counts more)
+          if (kTok == 128 && out_bytes == 16) {
+            const int n = n_w + (lane & 3) * 8;
+            const uint32_t ld_at = stage + (lane >> 2) * S::kOutPitch + (lane & 3) * 16;
+            uint16_t *dst = static_cast<uint16_t *>(p.out) + static_cast<size_t>(t.row0 + col0 + 8 * j0 + (lane >> 2)) * p.ld_out + n;
+#pragma unroll
+            for (int j = 0; j < S::kOutCols / 8; ++j, dst += 8 * p.ld_out) {
+              if (8 * (j0 + j) + (lane >> 2) >= ntok || n >= p.n) continue;
               uint32_t o[4];
-              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]) : "r"(stage + tok * S::kOutPitch + n * 2) : "memory");
-              uint16_t *dst = out + static_cast<size_t>(tok) * p.ld_out + n;
-              if (n_w + n + 8 <= p.n) {
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]) : "r"(ld_at + j * 8 * S::kOutPitch) : "memory");
+              if (n + 8 <= p.n) {
                 *reinterpret_cast<uint4 *>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
               } else {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                  if (n_w + n + e < p.n) dst[e] = static_cast<uint16_t>(o[e / 2] >> (16 * (e & 1)));
+                  if (n + e < p.n) dst[e] = static_cast<uint16_t>(o[e / 2] >> (16 * (e & 1)));
               }
             }
-          } else {
-            const int n = (lane & 15) * 2;
-            for (int tok = lane >> 4; tok < here; tok += 2) {
-              uint32_t o;
-              asm volatile("ld.shared.b32 %0, [%1];" : "=r"(o) : "r"(stage + tok * S::kOutPitch + n * 2) : "memory");
-              store_word16(out + static_cast<size_t>(tok) * p.ld_out + n, o, p.n - n_w - n, out_bytes);
-            }
+            continue;
+          }
+          const int here = min(ntok - 8 * j0, S::kOutCols), n = (lane & 15) * 2;
+          uint16_t *dst = static_cast<uint16_t *>(p.out) + static_cast<size_t>(t.row0 + col0 + 8 * j0 + (lane >> 4)) * p.ld_out + n_w + n;
+          for (int tok = lane >> 4; tok < here; tok += 2, dst += 2 * p.ld_out) {
+            uint32_t o;
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(o) : "r"(stage + tok * S::kOutPitch + n * 2) : "memory");
+            store_word16(dst, o, p.n - n_w - n, out_bytes);
           }
         }
       } else {
@@ -504,7 +516,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
       const GemmTile t = tile_of(it);
       const uint32_t base = smem_u32(ring_ptr);
       const int mine = (t.ntok - split + p.splits - 1) / p.splits;
-      add_up_splits<kScaleBlock, S::kThreads>(p, t, base, S::kPartPitch, mine, split, t.nb * kScaleBlock, out_bytes);
+      add_up_splits<kScaleBlock, S::kThreads, 1>(p, t, base, S::kPartPitch, mine, split, t.nb * kScaleBlock, out_bytes);
     }
     cluster_sync_all();   // no CTA leaves while another may still read its part
   }
@@ -838,7 +850,7 @@ fp8_gemm_wide_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
     if (first < n_items) {
       const GemmTile t = tile_at(p, s_tiles, first, n_nb);
       const int mine = (t.ntok - split + p.splits - 1) / p.splits;
-      add_up_splits<kWideN, kWideThreads>(p, t, ring, kWidePart, mine, split, t.nb * kWideN, out_bytes);
+      add_up_splits<kWideN, kWideThreads, 4>(p, t, ring, kWidePart, mine, split, t.nb * kWideN, out_bytes);
     }
     cluster_sync_all();   // no CTA leaves while another may still read its part
   }
