@@ -26,12 +26,34 @@ __device__ __forceinline__ float block_max(float v) {
   for (int off = kQuantLanes / 2; off; off >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
   return v;
 }
+// Two values side by side, two operations at a time, each rounded to nearest.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ float2 halves(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t v;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t v;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
 __device__ __forceinline__ uint4 encode16(const float (&v)[16], float inv) {
+  const uint64_t by = pair(inv, inv);
   uint32_t p[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i] * inv, v[4 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i + 2] * inv, v[4 * i + 3] * inv), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(halves(mul2(pair(v[4 * i], v[4 * i + 1]), by)), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(halves(mul2(pair(v[4 * i + 2], v[4 * i + 3]), by)), __NV_SATFINITE, __NV_E4M3);
     p[i] = lo | (hi << 16);
   }
   return make_uint4(p[0], p[1], p[2], p[3]);
@@ -39,8 +61,8 @@ __device__ __forceinline__ uint4 encode16(const float (&v)[16], float inv) {
 
 // gate * sigmoid(alpha * gate) * (up + 1) with the gate clamped from above and up on both sides (ACT_SWIGLU), or
 // gate * sigmoid(gate) * up (ACT_SILU_MUL); `rate` is -alpha * log2(e).  Minimum and maximum keep a NaN.  The fast exponential
-// and reciprocal are off by 2^-20 at |alpha * gate| = 8 and 2^-18 at 32, next to a code's half step of 2^-4: with expf and a
-// rounded division 17.7 M values took 46 us, the instructions being the bound.
+// and reciprocal are off by 2^-20 at |alpha * gate| = 8 and 2^-18 at 32, next to a code's half step of 2^-4: 30 to 40 of 17.7 M codes
+// are not those of 64 bits, as many as with expf and a rounded division, which took 37 us for 20.
 __device__ __forceinline__ float min_nan(float a, float b) {
   float r;
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -51,20 +73,30 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-__device__ __forceinline__ float over_one_plus_exp2(float x, float t) {   // x / (1 + 2^t)
-  float e, r;
+__device__ __forceinline__ float exp2_fast(float t) {
+  float e;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-  return x * r;
+  return e;
+}
+__device__ __forceinline__ float rcp_fast(float d) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+  return r;
 }
 template <int kAct>
-__device__ __forceinline__ float gated(float gate, float up, float limit, float rate) {
+__device__ __forceinline__ float2 gated(float gate0, float gate1, float up0, float up1, float limit, float rate) {
   if (kAct == MOE_ACT_SWIGLU) {
-    gate = min_nan(gate, limit);
-    up = max_nan(min_nan(up, limit), -limit);
-    return over_one_plus_exp2(gate, rate * gate) * (up + 1.f);
+    gate0 = min_nan(gate0, limit);
+    gate1 = min_nan(gate1, limit);
+    up0 = max_nan(min_nan(up0, limit), -limit);
+    up1 = max_nan(min_nan(up1, limit), -limit);
   }
-  return over_one_plus_exp2(gate, rate * gate) * up;
+  const uint64_t gate = pair(gate0, gate1), one = pair(1.f, 1.f);
+  uint64_t up = pair(up0, up1);
+  if (kAct == MOE_ACT_SWIGLU) up = add2(up, one);
+  const float2 t = halves(mul2(gate, pair(rate, rate)));
+  const float2 d = halves(add2(pair(exp2_fast(t.x), exp2_fast(t.y)), one));
+  return halves(mul2(mul2(gate, pair(rcp_fast(d.x), rcp_fast(d.y))), up));
 }
 
 // Sixteen values of a row as they lie in memory: consecutive ones in 16-byte loads, or every eighth (eight lanes read neighbours).
@@ -110,7 +142,7 @@ __device__ __forceinline__ void write_spread(uint8_t *p, int n, uint4 q) {
 __device__ __forceinline__ float finite_max(const float (&v)[16], float m) {
   float a = m;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) a = fmaxf(a, fabsf(v[i]));   // drops a NaN
+  for (int i = 0; i < 16; i += 2) asm("max.abs.f32 %0, %0, %1, %2;" : "+f"(a) : "f"(v[i]), "f"(v[i + 1]));   // drops a NaN
   if (a < __int_as_float(0x7f800000)) return a;
 #pragma unroll
   for (int i = 0; i < 16; ++i)
@@ -119,9 +151,11 @@ __device__ __forceinline__ float finite_max(const float (&v)[16], float m) {
 }
 
 // Eight lanes per block of 128 columns, sixteen columns each; the (row, block) pairs of a call are dealt to the groups of lanes.
-// Bound by instructions (addresses, places, the two quotients of a block cost the same whatever a lane converts): with eight
-// columns a lane 6144 x 2880 values through SwiGLU took 24 us, 1856 rows to four places each 8.5 us; they take 20.0 and 6.7.  More
-// pairs of a thread under way together cost registers and time; four CTAs to an SM in place of five 21.5 us.
+// Bound by instructions (addresses, places, the two quotients of a block cost the same whatever a lane converts; two values to an
+// instruction where there is one).  6144 x 2880 values through SwiGLU 18.1 us, 1856 rows to four places each 6.5; with eight columns a
+// lane 24 and 8.5, without the pairs of values 19.0, with four CTAs to an SM in place of five 19.5 and 7.4.  More pairs of a thread
+// under way together cost registers and time.  A grid of up to 16 CTAs an SM: with 5, 2048 x 7168 to eight places takes 30.5 us
+// instead of 26.6, with 40 the SwiGLU 19.1.
 constexpr int kQuantThreads = 256, kQuantGroups = kQuantThreads / kQuantLanes, kPlaces = 4;
 
 template <class T, int kAct, bool kWideIn>
@@ -135,9 +169,17 @@ quantize_fp8_kernel(const T *x, unsigned ld_x, int rows, int cols, unsigned n_bl
   const unsigned units = static_cast<unsigned>(live) * n_blocks;      // (row, block) pairs; the host bounds rows * n_blocks
   const unsigned stride = gridDim.x * kQuantGroups;
   // (the groups of a warp leave together: the shuffles are the whole warp's)
-  for (unsigned unit = blockIdx.x * kQuantGroups + threadIdx.x / kQuantLanes; __any_sync(0xffffffffu, unit < units); unit += stride) {
+  const unsigned row_step = stride / n_blocks, kb_step = stride - row_step * n_blocks;
+  unsigned unit = blockIdx.x * kQuantGroups + threadIdx.x / kQuantLanes, at_row = unit / n_blocks, at_kb = unit - at_row * n_blocks;
+  auto next = [&]() {
+    unit += stride;
+    at_row += row_step;
+    at_kb += kb_step;
+    if (at_kb >= n_blocks) { at_kb -= n_blocks; ++at_row; }
+  };
+  for (; __any_sync(0xffffffffu, unit < units); next()) {
     const bool on = unit < units;
-    const unsigned row = on ? unit / n_blocks : 0, kb = on ? unit - row * n_blocks : n_blocks;   // no column of block n_blocks exists
+    const unsigned row = on ? at_row : 0, kb = on ? at_kb : n_blocks;   // no column of block n_blocks exists
     // a lane's columns: sixteen neighbours, or, where rows of x are not 16-byte aligned and in a last part of a block that is not made
     // of sixteens, every eighth
     const int left = cols - static_cast<int>(kb * kScaleBlock);
@@ -147,9 +189,13 @@ quantize_fp8_kernel(const T *x, unsigned ld_x, int rows, int cols, unsigned n_bl
     float v[16];
     int place[kPlaces];
 #pragma unroll
-    for (int j = 0; j < kPlaces; ++j) {
-      place[j] = -1;
-      if (on && j < static_cast<int>(fanout)) place[j] = pair_row != nullptr ? pair_row[static_cast<size_t>(row) * fanout + j] : static_cast<int>(row);
+    for (int j = 0; j < kPlaces; ++j) place[j] = -1;
+    if (pair_row == nullptr) {
+      if (on) place[0] = static_cast<int>(row);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kPlaces; ++j)
+        if (on && j < static_cast<int>(fanout)) place[j] = pair_row[static_cast<size_t>(row) * fanout + j];
     }
     if (kAct == MOE_ACT_NONE) {
       Raw16<T> a;
@@ -172,13 +218,18 @@ quantize_fp8_kernel(const T *x, unsigned ld_x, int rows, int cols, unsigned n_bl
       }
       if (kAct == MOE_ACT_SWIGLU && whole) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          v[i] = gated<kAct>(a[2 * i], a[2 * i + 1], limit, rate);
-          v[i + 8] = gated<kAct>(b[2 * i], b[2 * i + 1], limit, rate);
+        for (int i = 0; i < 8; i += 2) {
+          const float2 p = gated<kAct>(a[2 * i], a[2 * i + 2], a[2 * i + 1], a[2 * i + 3], limit, rate);
+          const float2 q = gated<kAct>(b[2 * i], b[2 * i + 2], b[2 * i + 1], b[2 * i + 3], limit, rate);
+          v[i] = p.x; v[i + 1] = p.y;
+          v[i + 8] = q.x; v[i + 9] = q.y;
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = gated<kAct>(a[i], b[i], limit, rate);
+        for (int i = 0; i < 16; i += 2) {
+          const float2 p = gated<kAct>(a[i], a[i + 1], b[i], b[i + 1], limit, rate);
+          v[i] = p.x; v[i + 1] = p.y;
+        }
       }
     }
     const float m = block_max(finite_max(v, kAmaxFloor));
@@ -195,8 +246,11 @@ quantize_fp8_kernel(const T *x, unsigned ld_x, int rows, int cols, unsigned n_bl
       else if (static_cast<int>(lane * kQuantCols) < left) *reinterpret_cast<uint4 *>(dst + kb * kScaleBlock + lane * kQuantCols) = q;
       if (lane == 0) scales[static_cast<size_t>(static_cast<unsigned>(r)) * ld_scales + kb] = scale;
     };
+    put(place[0]);
+    if (fanout > 1) {
 #pragma unroll
-    for (int j = 0; j < kPlaces; ++j) put(place[j]);
+      for (int j = 1; j < kPlaces; ++j) put(place[j]);
+    }
     if (on)
       for (unsigned j = kPlaces; j < fanout; ++j) put(pair_row[static_cast<size_t>(row) * fanout + j]);
   }
