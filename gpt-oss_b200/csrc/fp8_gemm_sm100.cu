@@ -116,7 +116,7 @@ __device__ __forceinline__ void store_word16(uint16_t *dst, uint32_t w, int left
   }
 }
 
-constexpr int kMaxSplits = 4;   // CTAs of a cluster that share the reduction of a tile
+constexpr int kMaxSplits = 8;   // CTAs of a cluster that share the reduction of a tile
 
 // One tile: rows [row0, row0 + ntok) of group g against weight rows [128 nb, 128 nb + 128).
 struct GemmTile {
@@ -126,16 +126,16 @@ struct GemmTile {
 // A CTA's share of a split tile, kWidth output columns from n0: rows split, split + splits, ..., `mine` of them.  kAhead places of a
 // thread are under way together: a load from another CTA's shared memory takes about a microsecond.  The few rows of the narrow
 // kernel want less code instead: 128 x 4096 x 7168 13.6 us with one place, 14.2 with four.
-template <int kWidth, int kThreads, int kAhead>
+template <int kWidth, int kThreads, int kAhead, int kMost>
 __device__ __forceinline__ void add_up_splits(const Fp8GemmArgs &p, const GemmTile &t, uint32_t part, int pitch, int mine, int split, int n0, int out_bytes) {
   constexpr int kQuads = kWidth / 4;
   for (int e0 = threadIdx.x; e0 < mine * kQuads; e0 += kAhead * kThreads) {
-    float4 v[kAhead][kMaxSplits];
+    float4 v[kAhead][kMost];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       const int e = e0 + i * kThreads;
 #pragma unroll
-      for (int r = 0; r < kMaxSplits; ++r)
+      for (int r = 0; r < kMost; ++r)
         if (e < mine * kQuads && r < p.splits)
           v[i][r] = ld_cluster_f32x4(map_to_cta(part + 4u * ((split + e / kQuads * p.splits) * pitch + e % kQuads * 4), r));
     }
@@ -145,7 +145,7 @@ __device__ __forceinline__ void add_up_splits(const Fp8GemmArgs &p, const GemmTi
       if (e >= mine * kQuads) break;
       float4 sum = v[i][0];
 #pragma unroll
-      for (int r = 1; r < kMaxSplits; ++r)
+      for (int r = 1; r < kMost; ++r)
         if (r < p.splits) { sum.x += v[i][r].x; sum.y += v[i][r].y; sum.z += v[i][r].z; sum.w += v[i][r].w; }   // in the order of k
       float o[4] = {sum.x, sum.y, sum.z, sum.w};
       if (p.bias != nullptr) {
@@ -516,7 +516,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
       const GemmTile t = tile_of(it);
       const uint32_t base = smem_u32(ring_ptr);
       const int mine = (t.ntok - split + p.splits - 1) / p.splits;
-      add_up_splits<kScaleBlock, S::kThreads, 1>(p, t, base, S::kPartPitch, mine, split, t.nb * kScaleBlock, out_bytes);
+      if (p.splits <= 4) add_up_splits<kScaleBlock, S::kThreads, 1, 4>(p, t, base, S::kPartPitch, mine, split, t.nb * kScaleBlock, out_bytes);
+      else add_up_splits<kScaleBlock, S::kThreads, 1, kMaxSplits>(p, t, base, S::kPartPitch, mine, split, t.nb * kScaleBlock, out_bytes);
     }
     cluster_sync_all();   // no CTA leaves while another may still read its part
   }
@@ -850,7 +851,8 @@ fp8_gemm_wide_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
     if (first < n_items) {
       const GemmTile t = tile_at(p, s_tiles, first, n_nb);
       const int mine = (t.ntok - split + p.splits - 1) / p.splits;
-      add_up_splits<kWideN, kWideThreads, 4>(p, t, ring, kWidePart, mine, split, t.nb * kWideN, out_bytes);
+      if (p.splits <= 4) add_up_splits<kWideN, kWideThreads, 4, 4>(p, t, ring, kWidePart, mine, split, t.nb * kWideN, out_bytes);
+      else add_up_splits<kWideN, kWideThreads, 2, kMaxSplits>(p, t, ring, kWidePart, mine, split, t.nb * kWideN, out_bytes);
     }
     cluster_sync_all();   // no CTA leaves while another may still read its part
   }
@@ -905,28 +907,39 @@ struct GemmCall {
   Fp8GemmArgs p;
 };
 
-// CTAs that share the reduction of a tile where the call has at most `tiles`: 1, 2 or 4, as many as leave no SM without one.
-// Clusters of three or eight do not all fit the device at once although their CTAs would: 393 x 3011 x 6502 (48 tiles) in two 32
-// us, in three 42; 16 rows x 4096 x 7168 (32 tiles of 64 columns) in four 9.3 us, in eight 20.
+// CTAs that share the reduction of a tile where the call has at most `tiles`: 1, 2 or 4, as many as leave no SM without one, and 8 of
+// up to a dozen tiles with four blocks of k for each.  More clusters of eight, and any of three, do not all fit the device at once
+// although their CTAs would: 393 x 3011 x 6502 (48 tiles) in two 32 us, in three 42; 512 x 512 x 2048 (16 tiles) in four 8.5 us, in
+// eight 17.5; 16 rows of 1536 (12 tiles): 7168 deep 7.6 in four and 6.4 in eight, 2048 deep 5.2 and 5.6.
 int k_splits(long long tiles, int n_kb, int sm_count) {
   int splits = 1;
-  while (splits < kMaxSplits && tiles * splits * 2 <= sm_count && splits * 2 <= n_kb) splits *= 2;
-  return splits;
+  while (splits < 4 && tiles * splits * 2 <= sm_count && splits * 2 <= n_kb) splits *= 2;
+  return splits == 4 && tiles <= 12 && tiles * kMaxSplits <= sm_count && n_kb >= 4 * kMaxSplits ? kMaxSplits : splits;
 }
 
-// Which kernel, by the rows that a group has (on average: their numbers are on the device).  us, the kernel with 16 / 64 / 128
-// token columns / the wide one; one product of 4096 x 7168: 1 row 8.3 / 9.0 / 10.0 / 12.5, 16 rows 8.7 / 9.3 / 9.8 / 13.2,
-// 64 rows 18 / 11.5 / 11.4 / 14.7, 128 rows 33 / 17.0 / 13.2 / 16.9, 256 rows 63 / 25.7 / 18.9 / 18.3; 32 groups of 5760 x 2880:
-// 8 rows each 90 / 85 / 89 / 96, 32 rows 162 / 93 / 94 / 100, 64 rows 293 / 137 / 104 / 102, 96 rows 423 / 191 / 113 / 104.
-// A tile narrower than its group reads the weights again, from L2; with a tail of groups above the average, columns for twice
-// the average pay.
+// Which kernel.  Groups: by the rows that one has on average (their numbers are on the device).  us, the kernel with 64 / 128 token
+// columns / the wide one, 32 groups of 5760 x 2880: 8 rows each 85 / 89 / 96, 32 rows 93 / 94 / 100, 64 rows 137 / 104 / 102, 96 rows
+// 191 / 113 / 104.  A tile narrower than its group reads the weights again, from L2; with a tail of groups above the average, columns
+// for twice the average pay.
+// One product: 16 rows or fewer in the smallest tile (1 row of 4096 x 7168 8.2 us, in the next 9.0); else by what the blocks of k of the
+// busiest CTA cost, and the start and the end of a call.  64 / 128 / wide, measured: 128 x 4096 x 7168 17.0 / 12.9 / 16.9, 214 x 225 x
+// 7912 9.7 / 11.1 / 15.3, 256 x 1536 x 7168 16.4 / 13.3 / 13.9, 512 x 512 x 2048 8.0 / 8.5 / 11.0, 512 x 1536 x 7168 24.6 / 19.7 / 16.7,
+// 886 x 637 x 382 8.3 / 9.0 / 11.9, 1024 x 576 x 7168 24.8 / 19.7 / 16.7; the sums below are within 3 us of all of them.
 enum GemmForm { kForm16, kForm64, kForm128, kFormWide };
-GemmForm gemm_form(int rows, int n_groups, int n) {
-  const int per_group = (rows - 1) / n_groups + 1;
-  if (n_groups == 1 && per_group <= 16) return kForm16;
-  if (per_group <= (n_groups == 1 ? 64 : 32)) return kForm64;
-  if (per_group <= (n_groups == 1 ? 128 : 80) || n <= kScaleBlock) return kForm128;
-  return kFormWide;
+GemmForm gemm_form(int rows, int n_groups, int n, int n_kb, int sm_count) {
+  if (n_groups > 1) {
+    const int per_group = (rows - 1) / n_groups + 1;
+    return per_group <= 32 ? kForm64 : per_group <= 80 || n <= kScaleBlock ? kForm128 : kFormWide;
+  }
+  if (rows <= 16) return kForm16;
+  auto cost = [&](int tok, int width, double split_ends, double ends, double block) {
+    const long long tiles = ((rows - 1ll) / tok + 1) * ((n - 1ll) / width + 1);
+    const int splits = k_splits(tiles, n_kb, sm_count);
+    const long long rounds = (tiles * splits - 1) / sm_count + 1, blocks = (n_kb + splits - 1) / splits;
+    return (splits > 1 ? split_ends : ends) + block * static_cast<double>(rounds * blocks);
+  };
+  const double c64 = cost(64, kScaleBlock, 6.8, 6.8, 0.36), c128 = cost(128, kScaleBlock, 7.0, 7.0, 0.43), wide = cost(kWideTok, kWideN, 11.0, 8.0, 0.42);
+  return c64 <= c128 && c64 <= wide ? kForm64 : c128 <= wide ? kForm128 : kFormWide;
 }
 
 template <int kTok>
@@ -998,7 +1011,7 @@ int moe_gemm_fp8(moe_handle c, const uint8_t *a_dev, long long ld_a, const float
   p.bias = static_cast<const __nv_bfloat16 *>(bias_dev); p.out = out_dev; p.ld_out = static_cast<size_t>(ld_out);
   p.out_dtype = out_dtype; p.status = c->status;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const GemmForm form = gemm_form(rows, n_groups, n);
+  const GemmForm form = gemm_form(rows, n_groups, n, p.n_kb, c->sm_count);
   bool maps_ok = true;
   const cudaError_t e = form == kForm16    ? launch_fp8_gemm<16>(c, call, s, maps_ok)
                         : form == kForm64  ? launch_fp8_gemm<64>(c, call, s, maps_ok)

@@ -395,7 +395,7 @@ def check_product(p, buf, out):
 
 DENSE = [(1, 1, 1), (1, 128, 128), (1, 4096, 512), (3, 5, 17), (16, 256, 7168), (17, 130, 1000), (33, 2880, 2880), (64, 512, 129),
          (100, 200, 300), (127, 129, 128), (128, 256, 256), (129, 257, 640), (256, 1024, 96), (300, 5760, 384), (513, 384, 2944), (1000, 136, 1040),
-         (2049, 520, 272), (2500, 128, 200)]
+         (2049, 520, 272), (2500, 128, 200), (9, 300, 4100), (60, 130, 4096), (250, 100, 4300), (214, 225, 7912), (256, 1536, 14336), (300, 700, 2000)]
 
 
 @pytest.mark.parametrize("rows,n,k", DENSE)
@@ -416,7 +416,7 @@ def test_product_output_types_and_strides(rows, out, pad, pkg, handle):
 
 GROUPED = [([1], 96, 200), ([0, 0, 5, 0], 300, 256), ([8] * 8, 384, 512), ([3, 0, 17, 1, 0, 64, 2, 9], 260, 1040), ([130, 1, 0, 127, 128, 129], 520, 384),
            ([700, 5, 0, 300, 33], 256, 640), ([0, 0, 0], 128, 128), ([1] * 40, 144, 2880), ([257, 255, 256, 0, 31, 32, 33], 1152, 128),
-           ([16] * 200, 64, 64), ([1700, 5, 0, 2300, 33], 520, 384), ([1] * 1024, 130, 144), ([1900, 0, 300], 100, 256)]
+           ([16] * 200, 64, 64), ([1700, 5, 0, 2300, 33], 520, 384), ([1] * 1024, 130, 144), ([1900, 0, 300], 100, 256), ([9, 11], 300, 4200), ([0, 100, 90], 260, 5000)]
 
 
 @pytest.mark.parametrize("counts,n,k", GROUPED)
