@@ -20,8 +20,8 @@ namespace moe {
 // values differ by 2^-20, or 2^-17 of that largest, and 2^-22 of their own magnitudes (twice that for sums of two), or where
 // both logits and both biases are equal: then the index decides.  A row with a closer call is done again in 64 bits.  Of 8192 rows
 // of 256 experts some 18 are: 10.4 us without them, 15.2 with them, which is the time of one such row at the end (eight
-// rounds on 64-bit keys 1.6 us, the exponentials 0.3; with the first rows sent through that code, to have it in the caches, 17.0).  Settling only the calls in doubt, with one
-// exponential a lane, took the same 15.2, and 0.6 us more on a single row.
+// rounds on 64-bit keys 1.6 us, the exponentials 0.3; with the first rows sent through that code, to have it in the caches, 17.0).
+// Settling only the calls in doubt, with one exponential a lane, took the same 15.2, and 0.6 us more on a single row.
 //
 // A warp per row; lane l owns the per_lane consecutive experts from l * per_lane, so that a lower lane is a lower index.
 // ---------------------------------------------------------------------------
