@@ -388,9 +388,9 @@ route_scored_kernel(const T *logits, size_t ld, const float *bias, int rows, moe
   float sum = 0.f;
   if ((rule.n_groups == 1 || group_lanes > 0) && select_fast(src, x, bias, b, rule, per_lane, group_lanes, lane, top, sum, sel)) {
     // weights of the selected from their logits, within a few roundings of 32 bits
-    float s = 0.f;
+    float s = 0.f, v = 0.f;
     if (sel >= 0) {
-      float v = to_f32(src[sel]);
+      v = to_f32(src[sel]);
       if (v > 3.402823466e38f) v = 3.402823466e38f;
       if (rule.score == MOE_SCORE_SOFTMAX) {
         const float d = v - top, r = d - v, lost = (v - (d - r)) - (top + r);   // v - top is d + lost exactly
@@ -400,11 +400,19 @@ route_scored_kernel(const T *logits, size_t ld, const float *bias, int rows, moe
         s = __fdiv_rn(1.f, 1.f + expf(-v));
       }
     }
-    if (rule.renormalise) {
-      const float all = warp_sum(s);
-      share = all > 0.f ? __fdiv_rn(s, all) : 0.f;
+    if (__all_sync(0xffffffffu, sel < 0 || s >= 7.888609052210118e-31f)) {   // 2^-100
+      if (rule.renormalise) {
+        const float all = warp_sum(s);
+        share = all > 0.f ? __fdiv_rn(s, all) : 0.f;
+      } else {
+        share = rule.score != MOE_SCORE_SOFTMAX ? s : sum > 0.f ? __fdiv_rn(s, sum) : 0.f;
+      }
     } else {
-      share = rule.score != MOE_SCORE_SOFTMAX ? s : sum > 0.f ? __fdiv_rn(s, sum) : 0.f;
+      // Scores next to the smallest normal number of 32 bits (a sigmoid below -69, a softmax whose bias selects as far below the
+      // largest logit) lose their places, or are all 0 where their quotients are not: 64 bits
+      if (sel >= 0) share = rule.score == MOE_SCORE_SOFTMAX ? exp(static_cast<double>(v) - static_cast<double>(top)) : 1.0 / (1.0 + exp(-static_cast<double>(v)));
+      const double all = rule.renormalise ? warp_sum(share) : rule.score == MOE_SCORE_SOFTMAX ? static_cast<double>(sum) : 1.0;
+      share = all > 0.0 ? share / all : 0.0;
     }
   } else {
     double s;

@@ -1,0 +1,76 @@
+"""Routing by scores where 32 bits are not enough, against the definition in 64 bits (fp8_reference.py).
+
+Tolerance of a weight, by arithmetic: scores that are normal numbers of 32 bits carry at most sixteen roundings of 2^-24 to the
+weight (score, sum, quotient, scale) = 2^-20 relative; rows with smaller scores are formed in 64 bits and rounded once, which below
+2^-126 is half of the smallest step, 2^-150.
+"""
+import math
+
+import pytest
+import torch
+
+import fp8_reference as ref
+from test_fp8_layer_gpu import TYPES, run_route
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def handle(pkg):
+    h = pkg.MoeBlock(64, 64, 8, max_rows=8)
+    yield h
+    h.synchronize()
+    h.close()
+
+
+def check(pkg, handle, x, bias, dtype="f32", **args):
+    """x and the biases on the CPU."""
+    x = x.to(TYPES[dtype])
+    got = run_route(pkg, handle, x.cuda(), None if bias is None else bias.cuda(), dtype=dtype, **args)
+    want = ref.route(x, bias, **args)
+    assert torch.equal(got[0], want[0])
+    far, bound = (got[1].double() - want[1]).abs(), want[1].abs() * 2.0 ** -20 + 2.0 ** -150
+    assert (far <= bound).all(), float((far / bound).max())
+    return want
+
+
+# ------------------------------------------------------------------------------------------------ small scores
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("renorm,scale", [(True, 1.0), (False, 1.0), (False, 2.0 ** 100)])
+@pytest.mark.parametrize("experts,groups", [(4, 1), (64, 1), (64, 8), (512, 4)])
+def test_sigmoid_weights_of_low_logits(experts, groups, renorm, scale, bias, dtype, pkg, handle):
+    """Every selected score is small: exp(-x) is near the largest of 32 bits, or past it."""
+    g = torch.Generator().manual_seed(experts + groups)
+    lows = torch.tensor([-60.0, -69.0, -80.0, -85.0, -87.0, -87.5, -88.5, -89.0, -90.0, -95.0, -100.0, -104.0, -110.0, -300.0, -600.0, -700.0])
+    x = lows[:, None] - 0.5 * torch.argsort(torch.rand(len(lows), experts, generator=g), dim=1).clamp(max=8)
+    b = 0.1 * torch.randn(experts, generator=g) if bias else None
+    check(pkg, handle, x, b, dtype, top_k=4, score="sigmoid", n_groups=groups, top_groups=max(1, groups // 2), group_top=2, renorm=renorm, scale=scale)
+
+
+def test_sigmoid_weights_of_the_smallest_rows(pkg, handle):
+    want = check(pkg, handle, torch.tensor([[-90.0, -91.0, -92.0, -93.0], [-87.5, -88.5, -89.0, -90.0]]), None, top_k=4, score="sigmoid")
+    assert (want[1].sum(1) - 1).abs().max() < 1e-12
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("renorm,scale", [(True, 2.5), (False, 1.0), (False, 2.0 ** 100)])
+@pytest.mark.parametrize("experts,groups", [(32, 1), (256, 8), (512, 32)])
+def test_softmax_weights_far_below_the_largest_logit(experts, groups, renorm, scale, dtype, pkg, handle):
+    """A bias selects experts whose logits lie 30 to 600 below the row's largest."""
+    g = torch.Generator().manual_seed(experts)
+    below = torch.tensor([30.0, 50.0, 68.0, 70.0, 80.0, 86.0, 87.0, 88.0, 90.0, 100.0, 104.0, 110.0, 200.0, 400.0, 600.0])
+    x = torch.randn(len(below), experts, generator=g)
+    chosen = torch.argsort(torch.rand(experts, generator=g))[:6]
+    b = 0.01 * torch.randn(experts, generator=g)
+    b[chosen] = 3.0 + 0.25 * torch.arange(6)
+    x[:, chosen] = 0.5 * torch.randn(len(below), 6, generator=g) - below[:, None]
+    check(pkg, handle, x, b, dtype, top_k=4, score="softmax", n_groups=groups, top_groups=max(1, groups // 2), renorm=renorm, scale=scale)
+
+
+def test_softmax_weights_below_a_largest_logit_whose_expert_is_off(pkg, handle):
+    x = torch.tensor([[0.0, -120.0, -121.0, -122.0, -125.0, -300.0, -301.0, -302.0], [500.0, 1.0, 0.5, 0.25, 0.0, -1.0, -2.0, -3.0]])
+    b = torch.zeros(8)
+    b[0] = -math.inf
+    for renorm in (True, False):
+        check(pkg, handle, x, b, top_k=4, score="softmax", renorm=renorm)
