@@ -17,10 +17,11 @@ namespace moe {
 // no longer tell scores apart (a sigmoid above 16, logits within 1e-9) is the order not theirs.  With a bias a sigmoid in 32 bits
 // is off by less than 2^-21 (s (1 - s) times the exponential's (2 + 1.2 |x|) 2^-23, and the roundings of sum and quotient), a
 // softmax by less than 2^-18 of the row's largest (exponentials, a sum of up to 512, a quotient); so an order is certain where two
-// values differ by 2^-20, or 2^-17 of that largest, and 2^-22 of their own magnitudes (twice that for sums of two), or where
-// both logits and both biases are equal: then the index decides.  A row with a closer call is done again in 64 bits.  Of 8192 rows
-// of 256 experts some 18 are: 10.4 us without them, 15.2 with them, which is the time of one such row at the end (eight
-// rounds on 64-bit keys 1.6 us, the exponentials 0.3; with the first rows sent through that code, to have it in the caches, 17.0).
+// values differ by 2^-20, or 2^-17 of that largest, and 2^-22 of their own magnitudes (sums of two by twice that, and by twice
+// 2^-22 of their parts' magnitudes, which may have opposite signs), or where both logits and both biases are equal: then the index
+// decides.  A row with a closer call is done again in 64 bits.  Of 8192 rows of 256 experts some 18 are: 10.4 us without them, 15.2
+// with them, which is the time of one such row at the end (eight rounds on 64-bit keys 1.6 us, the exponentials 0.3; with the first
+// rows sent through that code, to have it in the caches, 17.0).
 // Settling only the calls in doubt, with one exponential a lane, took the same 15.2, and 0.6 us more on a single row.
 //
 // A warp per row; lane l owns the per_lane consecutive experts from l * per_lane, so that a lower lane is a lower index.
@@ -170,11 +171,10 @@ __device__ __forceinline__ bool select_fast(const T *src, const float (&x)[kPer]
   constexpr float lost = kPlace * 1.1920928955078125e-07f;                        // 2^-23 a place
   constexpr float rel = lost + 2.384185791015625e-07f;                            // and 2^-22
   const float close = softmax ? over * 7.62939453125e-06f : 9.5367431640625e-07f;   // 2^-17, 2^-20
-  auto far_apart = [&](float a, float c, float twice) { return a - c > twice * (close + rel * (fabsf(a) + fabsf(c))); };
   // the order of two keys (the first is not the smaller) is that of 64 bits
   auto certain = [&](unsigned ka, unsigned kc) {
     const float a = value(ka), c = value(kc);
-    if (bias != nullptr) return far_apart(a, c, 1.f);
+    if (bias != nullptr) return a - c > close + rel * (fabsf(a) + fabsf(c));
     return (softmax ? a > top - 600.f : c < 16.f && a > -600.f) && a - c > 1e-9f + (kExact ? 0.f : lost * (fabsf(a) + fabsf(c)));
   };
   bool settled = true;
@@ -185,16 +185,20 @@ __device__ __forceinline__ bool select_fast(const T *src, const float (&x)[kPer]
     k2 = __shfl_sync(0xffffffffu, k2, lane * group_lanes & 31) & ~kPlace;
     if (lane >= rule.n_groups) k1 = k2 = 0;
     unsigned worth = k1;
-    float off = 0.f;   // how far a sum may be off for what its logits lost
+    float off = 0.f;   // how far a sum may be off for its parts' roundings and for what their logits lost
     const bool sums = rule.group_top == 2;
     if (sums && k1 != 0) {
       auto part = [&](unsigned k) {
         if (k == 0) return 0.f;
         const float v = value(k);
-        if (bias != nullptr) return v;
-        const float s = score(v) * over, d = lost * fabsf(v);
-        if (!kExact) off += d < 0.1f ? 1.1f * d * s : inf;
-        return s;
+        float p = v;
+        if (bias == nullptr) {
+          const float d = lost * fabsf(v);
+          p = score(v) * over;
+          if (!kExact) off += d < 0.1f ? 1.1f * d * p : inf;
+        }
+        off += 2.f * rel * fabsf(p);
+        return p;
       };
       worth = ordered_key(part(k1) + part(k2));
     }
@@ -207,7 +211,7 @@ __device__ __forceinline__ bool select_fast(const T *src, const float (&x)[kPer]
       if (worth != 0 && wa != 0) {
         const unsigned hi = max(worth, wa), lo = min(worth, wa);
         const bool same = lane == in || (kExact && bias == nullptr && k1 == a1 && (!sums || k2 == a2));
-        settled = same || (sums ? far_apart(key_value(hi) - off - off_in, key_value(lo), 2.f) : certain(hi, lo));
+        settled = same || (sums ? key_value(hi) - key_value(lo) > 2.f * close + (off + off_in) : certain(hi, lo));
       }
     }
     if (!(stays >> (lane / group_lanes) & 1u)) {

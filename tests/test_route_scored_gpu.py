@@ -74,3 +74,38 @@ def test_softmax_weights_below_a_largest_logit_whose_expert_is_off(pkg, handle):
     b[0] = -math.inf
     for renorm in (True, False):
         check(pkg, handle, x, b, top_k=4, score="softmax", renorm=renorm)
+
+
+# ------------------------------------------------------------------------------------------------ groups by sums of two
+def opposite_signs(experts, groups, size_of_bias, rows=60):
+    """Groups worth nearly the same: their two best have biases near +- size_of_bias, whose sums lie a few 1e-6 apart."""
+    g = torch.Generator().manual_seed(experts + int(8 * size_of_bias))
+    size = experts // groups
+    b = torch.full((groups, size), -9.0 * size_of_bias)
+    at = torch.argsort(torch.rand(groups, size, generator=g), dim=1)[:, :2]
+    u, step = torch.rand(groups, 1, generator=g), 4e-6 * (torch.rand(groups, 1, generator=g) - 0.5)
+    b.scatter_(1, at, torch.cat([size_of_bias + u, step - size_of_bias - u], 1))
+    return 0.3 + 1e-5 * torch.randn(rows, experts, generator=g), b.view(-1)
+
+
+@pytest.mark.parametrize("size_of_bias", [0.5, 4.0, 10.0, 100.0])
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("experts,groups", [(32, 16), (256, 32), (512, 32)])      # 1, 8 and 16 experts a lane
+@pytest.mark.parametrize("share", [1, 2])
+def test_group_sums_of_opposite_signs(experts, groups, share, score, size_of_bias, pkg, handle):
+    x, b = opposite_signs(experts, groups, size_of_bias)
+    top_groups = 1 if share == 1 else groups // 2
+    # rows whose order the last places of 64 bits would decide are not asked for
+    s = torch.sigmoid(x.double()) if score == "sigmoid" else torch.softmax(x.double(), 1)
+    worth = (s + b.double()).view(len(x), groups, -1).topk(2, dim=2).values.sum(2).sort(dim=1, descending=True).values
+    x = x[worth[:, top_groups - 1] - worth[:, top_groups] > 1e-11]
+    assert len(x) > 50
+    check(pkg, handle, x, b, top_k=2, score=score, n_groups=groups, top_groups=top_groups, group_top=2)
+
+
+def test_group_sums_whose_parts_lose_their_last_places(pkg, handle):
+    """64 bits: group 1 is worth 0.210505247 + 1, group 0 0.210505009 + 1."""
+    b = torch.full((512,), -9.0)
+    b[0], b[1], b[16], b[17] = 2.9504035, -3.7398984, 2.4139395, -3.2034342
+    want = check(pkg, handle, torch.zeros(1, 512), b, top_k=2, score="sigmoid", n_groups=32, top_groups=1, group_top=2)
+    assert want[0].tolist() == [[16, 17]]
