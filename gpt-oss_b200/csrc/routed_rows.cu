@@ -10,7 +10,8 @@ namespace moe {
 // ---------------------------------------------------------------------------
 // Routing.  Of a row's logits x:  s = sigmoid(x), or softmax over the experts that are on;  p = s + bias;  the groups
 // with the highest sum of their group_top largest p stay;  the top_k largest p of what stays are selected, ties to the
-// lower index;  weight = s [/ sum of the selected s] * scale.  An expert is off where x or its bias is -inf or NaN.
+// lower index;  weight = s [/ sum of the selected s] * scale.  An expert is off where x is -inf or NaN.  Where its bias is, it is
+// not selected, but its x counts in the softmax: a bias does not change the scores.
 //
 // Which of two neighbouring p is larger is part of the answer, so the comparisons are those of 64 bits.  A row is tried in
 // 32 bits first.  Without a bias the scores are in the order of the logits, and these are compared; only where 64 bits themselves

@@ -248,9 +248,10 @@ typedef struct moe_route_rule {
 
 /* Routing by scores: logits_dev [rows, ld] of `dtype`, bias_dev fp32 [E] or NULL (it decides the selection, not the weights).
  * Of the top_groups groups worth most, the K experts with the largest s + bias are selected, largest first, equal ones by the
- * lower index; comparisons are made in 64 bits.  idx_dev i32 [rows, K], w_dev fp32 [rows, K].  An expert whose logit or bias is
- * -inf or NaN is off: it is never selected and takes no part in the softmax; +inf counts as the largest finite value.  Where
- * fewer than K experts are left the rest of the row is index -1 with weight 0. */
+ * lower index; comparisons are made in 64 bits.  idx_dev i32 [rows, K], w_dev fp32 [rows, K].  An expert whose logit is -inf or
+ * NaN is off: it is never selected and takes no part in the softmax; one whose bias is -inf or NaN is never selected, but its logit
+ * counts in the softmax as any other.  +inf counts as the largest finite value.  Where fewer than K experts are left the
+ * rest of the row is index -1 with weight 0. */
 int moe_route_scored(moe_handle h, const moe_route_rule *rule, const void *logits_dev, int dtype, long long ld,
                      const float *bias_dev, int rows, int *idx_dev, float *w_dev, void *stream);
 

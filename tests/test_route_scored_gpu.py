@@ -109,3 +109,25 @@ def test_group_sums_whose_parts_lose_their_last_places(pkg, handle):
     b[0], b[1], b[16], b[17] = 2.9504035, -3.7398984, 2.4139395, -3.2034342
     want = check(pkg, handle, torch.zeros(1, 512), b, top_k=2, score="sigmoid", n_groups=32, top_groups=1, group_top=2)
     assert want[0].tolist() == [[16, 17]]
+
+
+# ------------------------------------------------------------------------------------------------ biases that are not finite
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("groups", [1, 4])
+@pytest.mark.parametrize("experts", [32, 60, 256])
+@pytest.mark.parametrize("renorm", [False, True])
+def test_an_expert_off_by_its_bias_still_counts_in_the_softmax(score, groups, experts, renorm, pkg, handle):
+    """A bias decides the selection, not the weights: at -inf or NaN its expert is never selected, and the others' scores stay."""
+    g = torch.Generator().manual_seed(experts)
+    x, b = torch.randn(30, experts, generator=g), 0.1 * torch.randn(experts, generator=g)
+    x[::5, 3::7] = -math.inf
+    off = torch.zeros(experts, dtype=torch.bool)
+    off[::3] = True
+    b[::3], b[::6] = -math.inf, math.nan
+    args = dict(top_k=6, score=score, n_groups=groups, top_groups=max(1, groups // 2), group_top=2, renorm=renorm)
+    idx, w = check(pkg, handle, x, b, **args)
+    assert not off[idx[idx >= 0].long()].any()
+    if not renorm:
+        s = torch.sigmoid(x.double()) if score == "sigmoid" else torch.softmax(x.double(), 1)
+        found = idx >= 0
+        assert torch.allclose(w[found], s.gather(1, idx.clamp(min=0).long())[found], rtol=1e-12, atol=0)
