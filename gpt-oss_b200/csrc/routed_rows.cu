@@ -376,10 +376,15 @@ route_scored_kernel(const T *logits, size_t ld, const float *bias, int rows, moe
         if (i < per_lane && first + i < E) b[i] = bias[first + i];
     }
   }
+  if (bias != nullptr) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (b[i] > 3.402823466e38f) b[i] = 3.402823466e38f;   // +inf counts as the largest finite value (a NaN stays)
+  }
   float top = -inf;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    if (x[i] > 3.402823466e38f) x[i] = 3.402823466e38f;   // +inf counts as the largest finite value
+    if (x[i] > 3.402823466e38f) x[i] = 3.402823466e38f;
     if (x[i] != x[i]) x[i] = -inf;                         // NaN is off
     top = fmaxf(top, x[i]);
   }

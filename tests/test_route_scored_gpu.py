@@ -23,11 +23,11 @@ def handle(pkg):
     h.close()
 
 
-def check(pkg, handle, x, bias, dtype="f32", **args):
-    """x and the biases on the CPU."""
+def check(pkg, handle, x, bias, dtype="f32", want_bias=None, **args):
+    """x and the biases on the CPU; want_bias: what the biases count as."""
     x = x.to(TYPES[dtype])
     got = run_route(pkg, handle, x.cuda(), None if bias is None else bias.cuda(), dtype=dtype, **args)
-    want = ref.route(x, bias, **args)
+    want = ref.route(x, bias if want_bias is None else want_bias, **args)
     assert torch.equal(got[0], want[0])
     far, bound = (got[1].double() - want[1]).abs(), want[1].abs() * 2.0 ** -20 + 2.0 ** -150
     assert (far <= bound).all(), float((far / bound).max())
@@ -131,3 +131,17 @@ def test_an_expert_off_by_its_bias_still_counts_in_the_softmax(score, groups, ex
         s = torch.sigmoid(x.double()) if score == "sigmoid" else torch.softmax(x.double(), 1)
         found = idx >= 0
         assert torch.allclose(w[found], s.gather(1, idx.clamp(min=0).long())[found], rtol=1e-12, atol=0)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts,groups", [(32, 1), (32, 4), (60, 4), (256, 8)])
+@pytest.mark.parametrize("group_top", [1, 2])
+def test_an_infinite_bias_counts_as_the_largest_finite_one(score, experts, groups, group_top, pkg, handle):
+    """Two of them in a group are worth more than one, and one is worth what the largest finite bias is."""
+    g = torch.Generator().manual_seed(experts + group_top)
+    x, b = torch.randn(20, experts, generator=g), 0.1 * torch.randn(experts, generator=g)
+    size, most = experts // groups, torch.finfo(torch.float32).max
+    b[1] = math.inf
+    b[2 * size % experts + 2], b[2 * size % experts + 4] = math.inf, most
+    b[-1] = most
+    check(pkg, handle, x, b, want_bias=b.clamp(max=most), top_k=4, score=score, n_groups=groups, top_groups=1, group_top=group_top)
