@@ -172,10 +172,19 @@ __device__ __forceinline__ void add_up_splits(const Fp8GemmArgs &p, const GemmTi
 __device__ __forceinline__ int group_begin(const Fp8GemmArgs &p, int g) { return p.offsets == nullptr ? 0 : min(max(p.offsets[g], 0), p.rows); }
 __device__ __forceinline__ int group_end(const Fp8GemmArgs &p, int g) { return p.offsets == nullptr ? p.rows : min(max(p.offsets[g + 1], 0), p.rows); }
 
+// Token tiles of a group of cnt rows, and the rows of each of them: equal but for the last, in steps of 16.  (Unsigned: cnt may be
+// near 2^31.)
+__host__ __device__ constexpr int tiles_of(int cnt, unsigned tok) { return static_cast<int>((static_cast<unsigned>(cnt > 0 ? cnt : 0) + tok - 1) / tok); }
+__host__ __device__ constexpr int rows_of_tile(unsigned cnt, unsigned tiles) { return static_cast<int>(((cnt + tiles - 1) / tiles + 15) / 16 * 16); }
+constexpr int kMostRows = 0x7fffff00;   // of a call, and columns: with a tile more an index still fits an int
+static_assert(tiles_of(0, 64) == 0 && tiles_of(-5, 64) == 0 && tiles_of(1, 64) == 1 && tiles_of(64, 64) == 1 && tiles_of(65, 64) == 2, "tiles");
+static_assert(rows_of_tile(1, 1) == 16 && rows_of_tile(16, 1) == 16 && rows_of_tile(65, 2) == 48 && rows_of_tile(129, 2) == 80, "rows of a tile");
+static_assert(rows_of_tile(kMostRows, tiles_of(kMostRows, 64)) == 64 && rows_of_tile(kMostRows, tiles_of(kMostRows, 128)) == 128, "the largest call");
+
 // s_tiles[g] = token tiles of the groups before g, g = 0..n_groups.  Called by all threads, ends with a barrier.
 template <int kTok>
 __device__ __forceinline__ void count_tiles(const Fp8GemmArgs &p, int *s_tiles) {
-  for (int g = threadIdx.x; g < p.n_groups; g += blockDim.x) s_tiles[g + 1] = (max(group_end(p, g) - group_begin(p, g), 0) + kTok - 1) / kTok;
+  for (int g = threadIdx.x; g < p.n_groups; g += blockDim.x) s_tiles[g + 1] = tiles_of(group_end(p, g) - group_begin(p, g), kTok);
   __syncthreads();
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
@@ -215,7 +224,7 @@ __device__ __forceinline__ GemmTile tile_at(const Fp8GemmArgs &p, const int *s_t
   const int tiles = s_tiles[lo + 1] - s_tiles[lo];
   const int local = item - s_tiles[lo] * n_nb;
   const int begin = group_begin(p, lo), cnt = group_end(p, lo) - begin;
-  const int per = ((cnt + tiles - 1) / tiles + 15) / 16 * 16;
+  const int per = rows_of_tile(cnt, tiles);
   if (tiles <= kRunTiles) {
     const int nb = local / tiles, row = (local - nb * tiles) * per;
     return GemmTile{lo, nb, begin + row, min(per, cnt - row)};
@@ -997,6 +1006,7 @@ int moe_gemm_fp8(moe_handle c, const uint8_t *a_dev, long long ld_a, const float
     return op_fail(c, MOE_ERR_INVALID, "moe_gemm_fp8: %d x %d x %d, output type %d, strides %lld, %lld, %lld, %lld", rows, n, k, out_dtype, ld_a, ld_sa, ld_b, ld_out);
   if (n_groups < 1 || n_groups > 1024 || (!offsets_dev && n_groups != 1))
     return op_fail(c, MOE_ERR_INVALID, "moe_gemm_fp8: %d groups%s", n_groups, offsets_dev ? "" : " without offsets");
+  if (rows > kMostRows || n > kMostRows) return op_fail(c, MOE_ERR_INVALID, "moe_gemm_fp8: %d rows x %d columns in one call", rows, n);
   if (ld_a % 16 || ld_b % 16 || !aligned_to(a_dev, 16) || !aligned_to(b_dev, 16))
     return op_fail(c, MOE_ERR_INVALID, "moe_gemm_fp8: codes need 16-byte aligned rows (strides %lld, %lld)", ld_a, ld_b);
   if (rows == 0) return MOE_OK;

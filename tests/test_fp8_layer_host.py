@@ -112,3 +112,8 @@ def test_no_rows_is_a_call_that_does_nothing(pkg, handle):
     assert lib.moe_quantize_fp8_blocks(handle, None, 0, 64, 0, 8, 64, None, 64, None, None) == 0
     assert lib.moe_gemm_fp8(handle, *{**GEMM, "rows": 0, "a": 0, "out": 0}.values(), None) == 0
     assert lib.moe_combine_pairs(handle, *{**COMBINE, "rows": 0, "out": 0}.values(), None) == 0
+
+
+@pytest.mark.parametrize("change", [dict(rows=2 ** 31 - 255), dict(rows=2 ** 31 - 1), dict(n=2 ** 31 - 255, ld_out=2 ** 31), dict(n=2 ** 31 - 1, ld_out=2 ** 31)])
+def test_gemm_of_more_rows_or_columns_than_an_index_holds(change, pkg, handle):
+    refused(pkg, handle, pkg.lib().moe_gemm_fp8(handle, *{**GEMM, **change}.values(), None), "moe_gemm_fp8", "in one call")
