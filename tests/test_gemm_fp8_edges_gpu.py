@@ -1,7 +1,10 @@
-"""The FP8 product at the ends of its range."""
+"""The FP8 product beside values that are not finite, and output rows of 16-byte pieces that end inside one."""
+import math
+
 import pytest
 import torch
 
+import fp8_reference as ref
 from test_fp8_layer_gpu import check_product, make_product, run_product
 
 pytestmark = pytest.mark.gpu
@@ -13,6 +16,48 @@ def handle(pkg):
     yield h
     h.synchronize()
     h.close()
+
+
+# rows, n, k, rows of the groups: 16, 64 and 128 token columns and the wide form, whole and split over clusters of two, four and eight
+SHAPES = [(12, 200, 300, None), (16, 256, 7168, None), (40, 260, 1040, None), (214, 225, 7912, None), (200, 1030, 2000, None), (512, 1536, 1024, None),
+          (2100, 520, 300, None), (60, 300, 640, [20, 0, 25, 15]), (300, 200, 300, [120, 0, 80, 100]), (700, 520, 400, [300, 0, 250, 150])]
+
+
+@pytest.mark.parametrize("rows,n,k,counts", SHAPES)
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_scales_that_are_not_finite_reach_what_they_scale(rows, n, k, counts, value, pkg, handle):
+    """A row's scale: that row's outputs.  A block's scale: the block's columns in the rows of its group."""
+    groups = len(counts) if counts else 1
+    p = make_product(5, rows, n, k, groups=groups, counts=counts)
+    clean = run_product(pkg, handle, p, "f32")
+    bad, block, group = rows // 2, (n - 1) // 128, groups - 1
+    p["sa"][bad, ref.blocks(k) // 2] = value
+    p["sb"][group, block, ref.blocks(k) - 1] = value
+    got = run_product(pkg, handle, p, "f32")
+    hit = torch.zeros(rows, n, dtype=torch.bool, device="cuda")
+    hit[bad] = True
+    first = int(p["offsets"][group]) if counts else 0
+    hit[first:, 128 * block:] = True
+    assert torch.equal(got[~hit], clean[~hit])
+    assert not got[hit].isfinite().any()      # (a sum of 128 random products is not zero: no inf x 0)
+
+
+@pytest.mark.parametrize("rows,k", [(9, 300), (60, 640), (120, 2000), (200, 4096), (700, 400), (5000, 200)])
+@pytest.mark.parametrize("n", [257, 260, 262, 519])
+@pytest.mark.parametrize("out", ["f16", "bf16", "f32"])
+def test_aligned_output_rows_that_end_inside_a_piece(rows, n, k, out, pkg, handle):
+    """Rows 16-byte aligned, columns not made of 16-byte pieces: what lies between the last column and the next row stays."""
+    p = make_product(n, rows, n, k, bias=True)
+    p["sa"] *= 0.01          # inside the range of fp16
+    check_product(p, run_product(pkg, handle, p, out, ld_out=(n + 7) // 8 * 8 + 8), out)
+
+
+@pytest.mark.parametrize("n", [130, 262])
+@pytest.mark.parametrize("out", ["bf16", "f32"])
+def test_aligned_output_rows_of_groups_that_end_inside_a_piece(n, out, pkg, handle):
+    for counts in ([5, 0, 20], [130, 1, 0, 127, 128, 129]):
+        p = make_product(n, sum(counts), n, 384, groups=len(counts), counts=counts, bias=True)
+        check_product(p, run_product(pkg, handle, p, out, ld_out=(n + 7) // 8 * 8), out)
 
 
 def test_product_of_as_many_rows_as_an_index_holds(pkg, handle):
