@@ -9,6 +9,7 @@
 // written at several places (the rows of a token's experts): the values are read and converted once.
 #include <cuda_fp8.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "fp8_layer.cuh"
@@ -334,7 +335,8 @@ int moe_quantize_fp8(moe_handle c, const void *x_dev, int dtype, long long ld_x,
   // wide accesses: rows of 16-byte pieces (with MOE_ACT_SILU_MUL the second half of a row of x too)
   const int wide_in = aligned_to(x_dev, 16) && ld_x * size % 16 == 0 && (act != MOE_ACT_SILU_MUL || static_cast<long long>(cols) * size % 16 == 0);
   const int wide_out = aligned_to(codes_dev, 16) && ld_codes % 16 == 0;
-  const float rate = -1.44269504088896341f * (act == MOE_ACT_SWIGLU ? alpha : 1.f);
+  // (an alpha whose rate would be infinite: gates next to 0 are below the smallest maximum, but 0 * inf would be a NaN)
+  const float rate = std::clamp(-1.44269504088896341f * (act == MOE_ACT_SWIGLU ? alpha : 1.f), -3.402823466e38f, 3.402823466e38f);
   const unsigned grid = static_cast<unsigned>(std::min<long long>((units + kQuantGroups - 1) / kQuantGroups, static_cast<long long>(c->sm_count) * 16));
   auto go = [&](auto type, auto kernel) {
     using T = decltype(type);
