@@ -17,12 +17,13 @@
 // scales then serves four packed multiply-adds.  With a row per thread every scale of the tile is loaded in every thread, and a
 // block of 128 x 128 took 700 cycles for its multiply-adds instead of 120, although the tensor-memory loads of fragments are
 // slower (128 cycles of a quadrant for 64 columns, 35 for rows).  Bound by HBM: 256 rows over 32 experts of 5760 x 2880 85 us =
-// 6.3 TB/s.  One decode step (16 x 4096 x 7168) 8.6 us for the 4.5 that its weights take: launch, 14 blocks of k, and the sum
-// of four CTAs' parts.
+// 6.3 TB/s in a graph, 92 called one after the other.  One decode step (16 x 4096 x 7168) 8.6 us in a graph, 9.8 called, for the 4.5
+// that its weights take: launch, 14 blocks of k, and the sum of four CTAs' parts.
 //
 // Many rows per group (fp8_gemm_wide_kernel).  128 token rows x 256 weight rows; the token rows are the M operand, so that sa * sb
-// is one number per thread and block.  8192 x 4096 x 7168 224 us = 2.1 PFLOP/s, 6144 rows over 32 experts of 5760 x 2880 175 us,
-// both at the power cap: the clock falls to 1.36 GHz.  In cycles a block of k takes 775 (dense) for 512 of tensor pipe; two
+// is one number per thread and block.  8192 x 4096 x 7168 263 us = 1.83 PFLOP/s, 6144 rows over 32 experts of 5760 x 2880 208 us,
+// called one after the other, at the power cap: the clock falls to 1.36 GHz (short runs in a graph begin at a higher one: 218 to 255
+// and 175; the figures below are of those).  In cycles a block of k takes 775 (dense) for 512 of tensor pipe; two
 // accumulators of 256 columns are all that tensor memory holds, and one comes back for its next block after the MMA (512), the
 // wait that sees it done (180), eight loads of 16 columns with their multiply-adds (600) and the wait of the MMA warp (150).
 // Measured and set aside: pairs of CTAs (cta_group::2, 256 x 256), which move a third less through shared memory, 226 us for the
@@ -916,7 +917,7 @@ struct GemmCall {
   Fp8GemmArgs p;
 };
 
-// CTAs that share the reduction of a tile where the call has at most `tiles`: 1, 2 or 4, as many as leave no SM without one, and 8 of
+// CTAs that share the reduction of a tile where the call has at most `tiles`: 1, 2 or 4, as many as give no SM more than one, and 8 of
 // up to a dozen tiles with four blocks of k for each.  More clusters of eight, and any of three, do not all fit the device at once
 // although their CTAs would: 393 x 3011 x 6502 (48 tiles) in two 32 us, in three 42; 512 x 512 x 2048 (16 tiles) in four 8.5 us, in
 // eight 17.5; 16 rows of 1536 (12 tiles): 7168 deep 7.6 in four and 6.4 in eight, 2048 deep 5.2 and 5.6.

@@ -229,8 +229,9 @@ int moe_route_static(moe_handle h, int layer, const void *t_dev, int rows, float
  *   -> moe_gemm_fp8 -> moe_combine_pairs.
  * All take device pointers on the handle's device and any sizes (the handle's own configuration plays no part), are ordered on
  * `stream`, allocate nothing, keep nothing between calls, can be captured into a graph, and may overlap one another on the GPU;
- * zero rows are a valid call that does nothing.  Strides (ld) count elements between rows.  Inputs and outputs of a call must
- * not overlap, except that moe_combine_pairs may write over its residual (same address, stride and type). */
+ * zero rows are a valid call that does nothing (of moe_group_pairs: that writes offsets of 0).  Strides (ld) count elements between
+ * rows.  Inputs and outputs of a call must not overlap, except that moe_combine_pairs may write over its residual (same address,
+ * stride and type). */
 enum { MOE_F32 = 0, MOE_BF16 = 1, MOE_F16 = 2 };
 enum { MOE_SCORE_SOFTMAX = 0, MOE_SCORE_SIGMOID = 1 };
 enum { MOE_ACT_NONE = 0, MOE_ACT_SWIGLU = 1, MOE_ACT_SILU_MUL = 2 };
@@ -270,9 +271,10 @@ int moe_group_pairs(moe_handle h, const int *idx_dev, int rows, int top_k, int n
  *   MOE_ACT_SILU_MUL  v[j] = x[j] * sigmoid(x[j]) * x[cols + j]
  * (`cols` counts v; with an activation x has 2 * cols columns).  Row t is written to the fanout rows pair_row_dev[t, 0..fanout)
  * of codes_dev [out_rows, ld_codes] and scales_dev [out_rows, ld_scales >= ceil(cols / 128)]; places outside [0, out_rows) are
- * left out.  Without pair_row_dev row t goes to row t.  n_rows_dev (i32, may be NULL) on the device says how many of the rows
- * exist; rows, and columns behind `cols`, that nothing is written to keep what they hold.  rows * ceil(cols / 128) must be below
- * 2^30 and every stride fit an int.  Rows of 16-byte pieces (x, codes) are read and written in those. */
+ * left out, and no two rows of x may name the same place.  Without pair_row_dev row t goes to row t.  n_rows_dev (i32, may be NULL)
+ * on the device says how many of the rows exist; rows, and columns behind `cols`, that nothing is written to keep what they hold.
+ * A sigmoid below 2^-126 counts as 0.  rows * ceil(cols / 128) must be below 2^30 and every stride fit an int.  Rows of 16-byte
+ * pieces (x, codes) are read and written in those. */
 int moe_quantize_fp8(moe_handle h, const void *x_dev, int dtype, long long ld_x, int rows, int cols, int act, float limit,
                      float alpha, const int *pair_row_dev, int fanout, int out_rows, const int *n_rows_dev, uint8_t *codes_dev,
                      long long ld_codes, float *scales_dev, long long ld_scales, void *stream);
