@@ -31,3 +31,23 @@ def test_swiglu_of_any_finite_alpha(alpha, dtype, cols, pkg, handle):
     # half a step of the code (its smallest is 2^-9) and 2^-16 for exponential, quotient and scale
     far = (codes.view(torch.float8_e4m3fn).double() * step - v).abs()
     assert (far <= v.abs() * (2.0 ** -4 + 2.0 ** -16) + step * 2.0 ** -10).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,cols,ld", [(128, 128, 128), (200, 300, 304), (130, 257, 260)])
+def test_blocks_beside_values_that_are_not_finite(rows, cols, ld, dtype, pkg, handle):
+    """A NaN becomes a NaN code, an infinity +-448, and the scale is that of the block's finite values."""
+    w = torch.randn(2, rows, ld, generator=torch.Generator().manual_seed(rows)).cuda().to(TYPES[dtype])
+    w[0, 3, 5], w[0, 7, 100], w[1, rows - 1, cols - 1] = float("nan"), float("inf"), -float("inf")
+    w[1, :, :128] = float("inf")      # blocks without a finite value
+    codes = torch.full((2, rows, ld), 0x55, dtype=torch.uint8, device="cuda")
+    scales = torch.empty(2, ref.blocks(rows), ref.blocks(cols), device="cuda")
+    handle.quantize_fp8_blocks(w.data_ptr(), kind(pkg, dtype), ld, 2, rows, cols, codes.data_ptr(), ld, scales.data_ptr(), stream())
+    x = w[:, :, :cols].float()
+    want, want_s = ref.quantise_blocks(torch.where(x.isfinite(), x, 0.0))
+    want = want.view(torch.uint8).clone()
+    want[x == float("inf")], want[x == -float("inf")], want[x.isnan()] = 0x7e, 0xfe, 0x7f
+    got = codes[:, :, :cols].contiguous()
+    got[x.isnan()] &= 0x7f
+    assert torch.equal(got, want) and torch.equal(scales, want_s)
+    assert (codes[:, :, cols:] == 0x55).all()
