@@ -602,6 +602,9 @@ __device__ __forceinline__ void copy_box(const Fp8GemmArgs &p, const uint8_t *bo
   }
 }
 
+// Boxes that leave by the copy engine: none, those that lie in the output whole, all.
+enum { kTiledNone = 0, kTiledWhole = 1, kTiledAll = 2 };
+
 // kSplit: a cluster of p.splits CTAs, blockIdx.y of them, shares the reduction of one tile.
 template <bool kSplit>
 __global__ void __launch_bounds__(kWideThreads, 1)
@@ -798,6 +801,7 @@ fp8_gemm_wide_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
       }
       // Through shared memory, a box of 32 rows x 128 bytes at a time: 64 16-bit columns or 32 fp32 ones.  Rows that all exist
       // leave by the copy engine while the next box, or tile, is under way, others (and outputs that it cannot address) by the warp.
+      // The engine writes whole 16-byte pieces, so a last box that ends inside one leaves by the warp too.
       const int rows_here = t.ntok - quad * 32, row_out = t.row0 + quad * 32;
       const bool by_copy = tiled_out && rows_here >= 32;
       if (!mbar_wait_warp(bfull(buf), bpar, abort_flag, p.status, ST_WAIT_AREADY)) { ok = false; break; }
@@ -820,7 +824,7 @@ fp8_gemm_wide_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
       auto leave = [&](int n, int box_cols) {
         fence_proxy_async_smem();
         __syncwarp();
-        if (by_copy) {
+        if (by_copy && (tiled_out == kTiledAll || n + box_cols <= p.n)) {
           if (lane == 0 && n < p.n) {
             tma_store_2d(&tm_out, n, row_out, out_smem);
             tma_store_commit();
@@ -982,9 +986,10 @@ cudaError_t launch_fp8_gemm_wide(moe_ctx *h, const GemmCall &c, cudaStream_t s, 
   const auto kernel = p.splits > 1 ? fp8_gemm_wide_kernel<true> : fp8_gemm_wide_kernel<false>;
   const cudaError_t e = allow_smem(h, reinterpret_cast<const void *>(kernel), kWideSmem, p.splits > 1 ? kSmemGemmWideSplit : kSmemGemmWide);
   if (e != cudaSuccess) return e;
-  // outputs through the copy engine: rows of 16-byte pieces
+  // outputs through the copy engine: rows 16-byte aligned
   CUtensorMap mo = ma;
-  const int tiled = out_alignment(c.p) == 16 && encode_out(&mo, c.p);
+  const int tiled = out_alignment(c.p) != 16 || !encode_out(&mo, c.p) ? kTiledNone
+                    : static_cast<long long>(c.p.n) * dtype_size(c.p.out_dtype) % 16 == 0 ? kTiledAll : kTiledWhole;
   const dim3 grid(static_cast<unsigned>(p.splits > 1 ? most : std::min<long long>(most, sm_count)), p.splits, 1);
   return launch_kernel(kernel, grid, kWideThreads, kWideSmem, s, true, p.splits > 1 ? p.splits : 0, ma, mb, mo, p, tiled, out_alignment(p));
 }

@@ -201,8 +201,9 @@ __device__ __forceinline__ void tma_load_5d_pair_hint(uint32_t dst, const CUtens
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(u), "r"(v), "l"(policy)
       : "memory");
 }
-// 2-D tile store, shared -> global; the tile may reach over the tensor's upper edges (what is outside is not written).  A
-// thread's stores since the last commit are a group; wait_read: shared memory may be written again, wait_all: written out.
+// 2-D tile store, shared -> global; the tile may reach over the tensor's upper edges.  What is outside is not written, but for the
+// rest of a 16-byte piece that the innermost edge lies in.  A thread's stores since the last commit are a group; wait_read: shared
+// memory may be written again, wait_all: written out.
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap *m, int x, int y, uint32_t src) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];"
                ::"l"(reinterpret_cast<uint64_t>(m)), "r"(src), "r"(x), "r"(y)

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import fp8_reference as ref
-from test_fp8_layer_gpu import check_product, make_product, run_product
+from test_fp8_layer_gpu import TYPES, check_product, kind, make_product, run_product, stream
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +77,25 @@ def test_product_of_as_many_rows_as_an_index_holds(pkg, handle):
     assert (between == between[0]).all()
     del large, out, between
     torch.cuda.empty_cache()
+
+
+# all but one in the form of many rows per group, whole: the copy engine writes pieces of 16 bytes
+WIDE = [(809, 146, 2, [300, 300, 209]), (2132, 129, 4, [700, 732, 700]), (4886, 410, 4, [1600, 1600, 1686]), (4707, 745, 1500, None), (2600, 1271, 1863, None),
+        (6000, 500, 1500, None), (9000, 257, 130, None), (3000, 515, 260, [1000, 0, 1999])]
+
+
+@pytest.mark.parametrize("rows,n,k,counts", WIDE)
+@pytest.mark.parametrize("out", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("beside", [0, 8, 40])
+def test_an_output_inside_a_wider_tensor(rows, n, k, counts, out, beside, pkg, handle):
+    """`beside` columns on its left, at least as many on its right; they stay, and so does what lies behind the last row."""
+    p = make_product(rows, rows, n, k, groups=len(counts) if counts else 1, counts=counts, bias=True)
+    p["sa"] *= 0.003         # inside the range of fp16
+    ld = (beside + n + 7) // 8 * 8 + beside
+    whole = torch.full((rows * ld + 64,), 77.0, dtype=TYPES[out], device="cuda")
+    view = whole[:rows * ld].view(rows, ld)[:, beside:]
+    handle.gemm_fp8(p["a"].data_ptr(), p["a"].shape[1], p["sa"].data_ptr(), p["sa"].shape[1], rows, p["b"].data_ptr(), p["b"].shape[2], p["sb"].data_ptr(), n, k,
+                    view.data_ptr(), kind(pkg, out), ld, bias_ptr=p["bias"].data_ptr(), n_groups=p["groups"],
+                    offsets_ptr=0 if p["offsets"] is None else p["offsets"].data_ptr(), stream=stream())
+    check_product(p, view, out)
+    assert (whole[rows * ld:] == 77).all() and (whole[:rows * ld].view(rows, ld)[:, :beside] == 77).all()
