@@ -145,3 +145,20 @@ def test_an_infinite_bias_counts_as_the_largest_finite_one(score, experts, group
     b[2 * size % experts + 2], b[2 * size % experts + 4] = math.inf, most
     b[-1] = most
     check(pkg, handle, x, b, want_bias=b.clamp(max=most), top_k=4, score=score, n_groups=groups, top_groups=1, group_top=group_top)
+
+
+# ------------------------------------------------------------------------------------------------ the sum of a softmax
+@pytest.mark.parametrize("experts", [128, 256, 512])
+@pytest.mark.parametrize("bias", [False, True])
+def test_weights_of_a_softmax_that_is_not_renormalised(experts, bias, pkg, handle):
+    """One logit of 0 and all others at the same distance: roundings of their exponentials and of the sum would all go one way.
+    Roundings of 2^-24: two of an exponential (one last place), once in the sum and once in the selected score, which takes one
+    more; the sum, the quotient and the scaled weight, one each: eight."""
+    d = torch.linspace(-16.0, -0.5, 20000, device="cuda")
+    x = d[:, None].repeat(1, experts)
+    x[:, 7] = 0
+    b = torch.zeros(experts, device="cuda") if bias else None
+    got = run_route(pkg, handle, x, b, 1, "softmax", renorm=False)
+    want = (1 / torch.exp(x.double()).sum(1, keepdim=True)).cpu()
+    assert (got[0] == 7).all()
+    assert ((got[1].double() - want).abs() <= want * 8 * 2.0 ** -24).all()
