@@ -801,7 +801,8 @@ fp8_gemm_wide_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
       }
       // Through shared memory, a box of 32 rows x 128 bytes at a time: 64 16-bit columns or 32 fp32 ones.  Rows that all exist
       // leave by the copy engine while the next box, or tile, is under way, others (and outputs that it cannot address) by the warp.
-      // The engine writes whole 16-byte pieces, so a last box that ends inside one leaves by the warp too.
+      // The engine writes whole 16-byte pieces, so a last box that ends inside one leaves by the warp too (8192 x 512 deep, rows of 4104
+      // bf16: 4104 columns 38.3 us, 4097 to 4103 39.7 to 40.6).
       const int rows_here = t.ntok - quad * 32, row_out = t.row0 + quad * 32;
       const bool by_copy = tiled_out && rows_here >= 32;
       if (!mbar_wait_warp(bfull(buf), bpar, abort_flag, p.status, ST_WAIT_AREADY)) { ok = false; break; }

@@ -288,9 +288,9 @@ int moe_quantize_fp8_blocks(moe_handle h, const void *w_dev, int dtype, long lon
  * products exact, sums in fp32, rounded once to out_dtype.  a_dev e4m3 [rows, ld_a], sa_dev [rows, ld_sa >= ceil(k / 128)],
  * b_dev e4m3 [n_groups, n, ld_b], sb_dev [n_groups, ceil(n / 128), ceil(k / 128)], bias_dev bf16 [n_groups, n] or NULL.
  * offsets_dev i32 [n_groups + 1] on the device, ascending: group g (<= 1024) is rows [offsets[g], offsets[g + 1]), output rows
- * in no group keep what they hold; NULL: one group, all rows.  rows and n are at most 2^31 - 256, ld_a and ld_b multiples of 16 and both
- * code tensors 16-byte aligned (MOE_ERR_INVALID otherwise); codes behind column k are not looked at.  Output rows of 16-byte pieces are
- * the fastest. */
+ * in no group, and what lies behind column n, keep what they hold; NULL: one group, all rows.  rows and n are at most 2^31 - 256, ld_a
+ * and ld_b multiples of 16 and both code tensors 16-byte aligned (MOE_ERR_INVALID otherwise); codes behind column k are not looked
+ * at.  Output rows of 16-byte pieces are the fastest. */
 int moe_gemm_fp8(moe_handle h, const uint8_t *a_dev, long long ld_a, const float *sa_dev, long long ld_sa, int rows,
                  const uint8_t *b_dev, long long ld_b, const float *sb_dev, int n, int k, int n_groups, const int *offsets_dev,
                  const void *bias_dev, void *out_dev, int out_dtype, long long ld_out, void *stream);
